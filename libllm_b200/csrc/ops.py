@@ -5,12 +5,13 @@ a tensor that is not on a CUDA device is an error."""
 from __future__ import annotations
 
 import ctypes
+import math
 from ctypes import c_float, c_int, c_longlong, c_void_p
 from typing import Optional
 
 import torch
 
-from ..errors import ExtensionError, UnsupportedError
+from ..errors import ExtensionError, InvalidArgError, UnsupportedError
 from . import build
 
 F32, BF16 = 0, 1
@@ -337,6 +338,191 @@ def sample(logits: torch.Tensor, temperature: float, top_k: int, top_p: float, u
           [c_void_p, c_longlong, c_int, c_int, c_float, c_int, c_float, c_void_p, c_void_p, c_void_p],
           _ptr(logits), logits.stride(0), logits.shape[0], logits.shape[1], float(temperature), int(top_k),
           float(top_p), _ptr(uniforms), _ptr(out), _stream())
+    return out
+
+
+def _same_device(*tensors) -> None:
+    """The tensors lie on the current device, where the launch goes."""
+    _on_gpu(*tensors)
+    current = torch.cuda.current_device()
+    for t in tensors:
+        if t is not None and t.device.index != current:
+            raise InvalidArgError(f"a tensor lies on '{t.device}', the launch goes to the current device 'cuda:{current}'")
+
+
+def _per_row(name: str, v, rows: int, *, positive: bool = False):
+    """A number for all rows, or a 32-bit tensor with one per row: (the tensor or None, the number)."""
+    if isinstance(v, torch.Tensor):
+        if v.dtype != torch.float32 or v.shape != (rows,) or not v.is_contiguous():
+            raise InvalidArgError(f"adjust_logits: {name} is a number or a contiguous float32 tensor with one per row ({rows})")
+        return v, 0.0
+    v = float(v)
+    if not math.isfinite(v) or (positive and v <= 0):
+        raise InvalidArgError(f"adjust_logits: {name} must be a finite{' positive' if positive else ''} number, got {v}")
+    return None, v
+
+
+_ADJUST_ARGS = [c_void_p, c_longlong, c_void_p, c_longlong, c_int, c_int, c_void_p, c_longlong, c_int, c_int, c_void_p, c_void_p, c_void_p, c_float,
+                c_void_p, c_float, c_void_p, c_float, c_void_p, c_longlong, c_void_p, c_longlong, c_void_p]
+
+
+def adjust_logits(logits: torch.Tensor, out: Optional[torch.Tensor] = None, history: Optional[torch.Tensor] = None,
+                  slots: Optional[torch.Tensor] = None, lengths: Optional[torch.Tensor] = None, repetition=1.0, presence=0.0, frequency=0.0,
+                  bias: Optional[torch.Tensor] = None, allowed: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Logits [B, V] as a request wants them sampled, in this order: every token that row b's history holds has its logit divided by
+    ``repetition`` where it is positive and multiplied by it elsewhere, and one that was drawn n > 0 times loses ``frequency`` n +
+    ``presence``; ``bias`` ([V] or [B, V]) is added; a token whose bit (v % 32 of word v / 32 of ``allowed``, int32 [words] or
+    [B, words]) is not set gets minus infinity, and a row that allows nothing is minus infinity throughout.
+
+    ``history`` [places, longest] int32: row b's sequence is the first ``lengths[b]`` entries (at most ``longest``) of place ``slots[b]`` (b
+    itself without slots; a place outside the history: an empty one), an id for a token that was drawn, ~id for one that a prompt brought; ids
+    outside the vocabulary count for nothing.  repetition (above 0), presence and frequency: a number, or a float32 tensor [B]; without a
+    history they do nothing.  ``out`` (new where None) may be ``logits`` itself, and no other tensor that overlaps it.  All 32-bit."""
+    if logits.dim() != 2 or logits.dtype != torch.float32 or (logits.shape[1] > 1 and logits.stride(1) != 1):
+        raise InvalidArgError("adjust_logits: logits are float32 [rows, vocabulary] with neighbouring columns")
+    B, V = logits.shape
+    if B > 65535 or V > 1 << 30:
+        raise UnsupportedError(f"adjust_logits: {B} rows of {V} logits are not taken")
+    if out is not None and (out.dtype != torch.float32 or out.shape != logits.shape or (V > 1 and out.stride(1) != 1) or (B > 1 and out.stride(0) < V)):
+        raise InvalidArgError("adjust_logits: out has the logits' shape and type, and rows of its own")
+    ldh = places = longest = 0
+    if history is not None:
+        if history.dim() != 2 or history.dtype != torch.int32 or (history.shape[1] > 1 and history.stride(1) != 1):
+            raise InvalidArgError("adjust_logits: the history is int32 [places, longest] with neighbouring entries")
+        places, longest = history.shape
+        ldh = history.stride(0)
+        for name, t in (("lengths", lengths), ("slots", slots)):
+            if t is None and name == "slots":
+                if B > places:
+                    raise InvalidArgError(f"adjust_logits: {B} rows without slots, the history has {places} places")
+            elif t is None or t.dtype != torch.int32 or t.shape != (B,) or not t.is_contiguous():
+                raise InvalidArgError(f"adjust_logits: {name} are contiguous int32 with one per row ({B})")
+        if places * longest == 0:
+            history = None                      # nothing was said
+    repetition, rep_all = _per_row("repetition", repetition, B, positive=True)
+    presence, pres_all = _per_row("presence", presence, B)
+    frequency, freq_all = _per_row("frequency", frequency, B)
+    ldb = lda = 0
+    if bias is not None:
+        if bias.dtype != torch.float32 or bias.shape not in ((V,), (B, V)) or (V > 1 and bias.stride(-1) != 1):
+            raise InvalidArgError(f"adjust_logits: the bias is float32 [{V}] or [{B}, {V}] with neighbouring columns")
+        ldb = bias.stride(0) if bias.dim() == 2 else 0
+    if allowed is not None:
+        words = (V + 31) // 32
+        if allowed.dtype != torch.int32 or allowed.shape not in ((words,), (B, words)) or (words > 1 and allowed.stride(-1) != 1):
+            raise InvalidArgError(f"adjust_logits: allowed is int32 [{words}] or [{B}, {words}] (a bit per token) with neighbouring words")
+        lda = allowed.stride(0) if allowed.dim() == 2 else 0
+    _same_device(logits, out, history, slots, lengths, repetition, presence, frequency, bias, allowed)
+    if out is None:
+        out = torch.empty(B, V, dtype=torch.float32, device=logits.device)
+    _call("logits", "llm_adjust_logits", _ADJUST_ARGS, _ptr(logits), logits.stride(0), _ptr(out), out.stride(0), B, V, _ptr(history), ldh, places, longest,
+          _ptr(slots), _ptr(lengths), _ptr(repetition), rep_all, _ptr(presence), pres_all, _ptr(frequency), freq_all, _ptr(bias), ldb, _ptr(allowed),
+          lda, _stream())
+    return out
+
+
+# ------------------------------------------------------------------ microscaled 4-bit floating point
+FP4_FORMATS = {"nvfp4": 0, "mxfp4": 1}
+
+
+class Fp4Matrix:
+    """A matrix [rows, cols] in four bits (csrc/fp4.cu says what lies where): codes, block scales and row scales in one piece of device
+    memory.  ``fp4_quantize`` makes one or fills one again."""
+    __slots__ = ("rows", "cols", "format", "data", "_at")
+
+    def __init__(self, rows: int, cols: int, format: str = "nvfp4", device=None):
+        if format not in FP4_FORMATS:
+            raise InvalidArgError(f"fp4: format '{format}' is not known ({' or '.join(FP4_FORMATS)})")
+        if rows < 0 or not 0 < cols <= 1 << 28:
+            raise InvalidArgError(f"fp4: a matrix of {rows} x {cols} is not taken")
+        self.rows, self.cols, self.format = rows, cols, format
+        codes = rows * ((cols + 31) // 32 * 16)
+        scales = (rows + 127) // 128 * ((cols + 255) // 256) * (2048 if format == "nvfp4" else 1024)
+        at = (codes + 511) // 512 * 512
+        self._at = (codes, at, at + scales, at + scales + 4 * rows)
+        self.data = torch.empty(max(self._at[3], 1), dtype=torch.uint8, device="cuda" if device is None else device)
+
+    @property
+    def device(self):
+        return self.data.device
+
+    @property
+    def nbytes(self) -> int:
+        return self._at[3]
+
+    @property
+    def codes(self) -> torch.Tensor:
+        """uint8 [rows, bytes of a row]: two codes a byte, the lower four bits first."""
+        return self.data[:self._at[0]].view(self.rows, -1) if self.rows else self.data.new_empty(0, (self.cols + 31) // 32 * 16)
+
+    @property
+    def scales(self) -> torch.Tensor:
+        """uint8, tiles of 128 rows x 4 blocks."""
+        return self.data[self._at[1]:self._at[2]]
+
+    @property
+    def row_scale(self) -> torch.Tensor:
+        return self.data[self._at[2]:self._at[3]].view(torch.float32)
+
+    def _pointers(self):
+        p = self.data.data_ptr()
+        return c_void_p(p), c_void_p(p + self._at[1]), c_void_p(p + self._at[2])
+
+
+_FP4_QUANTIZE_ARGS = [c_int, c_void_p, c_longlong, c_void_p, c_void_p, c_void_p, c_longlong, c_int, c_int, c_void_p]
+_FP4_DEQUANTIZE_ARGS = [c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_longlong, c_longlong, c_int, c_int, c_void_p]
+_FP4_GEMM_ARGS = [c_void_p] * 6 + [c_int, c_void_p, c_longlong, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p]
+
+
+def fp4_quantize(x: torch.Tensor, format: str = "nvfp4", out: Optional[Fp4Matrix] = None) -> Fp4Matrix:
+    """x [rows, cols] (bfloat16 or float32, any row stride) in four bits.  nvfp4: blocks of 16 along a row with e4m3 scales and a power of two
+    per row; mxfp4: blocks of 32 with powers of two.  A code is the nearest one, halves go to the even code, what is too large becomes the
+    largest.  A row that holds a NaN or an infinity becomes NaN throughout.  ``out``: a matrix of the same shape and format to fill."""
+    if x.dim() != 2 or (x.shape[1] > 1 and x.stride(1) != 1):
+        raise InvalidArgError("fp4_quantize: x is [rows, cols] with neighbouring columns")
+    dt = dtype_code(x.dtype)
+    rows, cols = x.shape
+    if format not in FP4_FORMATS:
+        raise InvalidArgError(f"fp4_quantize: format '{format}' is not known ({' or '.join(FP4_FORMATS)})")
+    if out is not None and (out.rows, out.cols, out.format) != (rows, cols, format):
+        raise InvalidArgError(f"fp4_quantize: out is {out.format} [{out.rows}, {out.cols}], x becomes {format} [{rows}, {cols}]")
+    _same_device(x, out.data if out is not None else None)
+    if out is None:
+        out = Fp4Matrix(rows, cols, format, x.device)
+    _call("fp4", "llm_fp4_quantize", _FP4_QUANTIZE_ARGS, dt, _ptr(x), x.stride(0), *out._pointers(), rows, cols, FP4_FORMATS[format], _stream())
+    return out
+
+
+def fp4_dequantize(q: Fp4Matrix, dtype: torch.dtype = torch.float32, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """What a matrix in four bits stands for, [rows, cols] float32 or bfloat16 (both hold it exactly where it is within
+    their range; an nvfp4 scale that was rounded up may take a value within 3 % of the largest number beyond it)."""
+    dt = dtype_code(dtype if out is None else out.dtype)
+    if out is not None and (out.shape != (q.rows, q.cols) or (q.cols > 1 and out.stride(1) != 1) or (q.rows > 1 and out.stride(0) < q.cols)):
+        raise InvalidArgError(f"fp4_dequantize: out is [{q.rows}, {q.cols}] with neighbouring columns and rows of its own")
+    _same_device(q.data, out)
+    if out is None:
+        out = torch.empty(q.rows, q.cols, dtype=dtype, device=q.device)
+    _call("fp4", "llm_fp4_dequantize", _FP4_DEQUANTIZE_ARGS, *q._pointers(), dt, _ptr(out), out.stride(0), q.rows, q.cols,
+          FP4_FORMATS[q.format], _stream())
+    return out
+
+
+def fp4_gemm(x: Fp4Matrix, w: Fp4Matrix, out: Optional[torch.Tensor] = None, out_dtype: torch.dtype = torch.float32) -> torch.Tensor:
+    """out[M, N] = x[M, K] @ w[N, K]^T of two matrices in the same format, on tcgen05 with block scales, 32-bit sums, for any sizes; the
+    result float32 or bfloat16.  Fast where w has many rows and x is the smaller of the two."""
+    if x.format != w.format or x.cols != w.cols:
+        raise InvalidArgError(f"fp4_gemm: {x.format} [{x.rows}, {x.cols}] and {w.format} [{w.rows}, {w.cols}] do not meet")
+    M, N = x.rows, w.rows
+    if max(M, N) >= 1 << 30:
+        raise UnsupportedError(f"fp4_gemm: {M} x {N} is not taken")
+    dt = dtype_code(out_dtype if out is None else out.dtype)
+    if out is not None and (out.shape != (M, N) or (N > 1 and out.stride(1) != 1) or (M > 1 and out.stride(0) < N)):
+        raise InvalidArgError(f"fp4_gemm: out is [{M}, {N}] with neighbouring columns and rows of its own")
+    _same_device(x.data, w.data, out)
+    if out is None:
+        out = torch.empty(M, N, dtype=out_dtype, device=w.device)
+    _call("fp4", "llm_fp4_gemm", _FP4_GEMM_ARGS, *x._pointers(), *w._pointers(), dt, _ptr(out), out.stride(0), M, N, x.cols,
+          FP4_FORMATS[x.format], 0, _ptr(tc_status(w.device)), _stream())
     return out
 
 

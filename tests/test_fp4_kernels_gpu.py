@@ -1,0 +1,255 @@
+"""Matrices in four bits against a plain 64-bit implementation: the codes and scales exactly, products within what 32-bit sums allow."""
+import pytest
+import torch
+
+import plain_four_bits as P
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+FORMATS = ["nvfp4", "mxfp4"]
+
+
+def ops():
+    from libllm_b200.csrc import ops as o
+    return o
+
+
+def rows_like(rows, cols, seed, dtype=torch.bfloat16, spread=6):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(rows, cols, generator=g) * torch.exp2(torch.randint(-spread, spread, (rows, 1), generator=g).float())
+    x[:, torch.rand(cols, generator=g) < 0.02] *= 30
+    return x.to(dtype)
+
+
+def same_values(x, format, got):
+    # An nvfp4 scale may be rounded up, so that a value within 3 % of the type's largest stands for more than the type holds: 255/256 2^128 has the
+    # row scale 2^117 and the block scale 340 -> 352, and 6 * 352 * 2^117 = 1.03 * 2^128 is infinite in 32 bits.  All else is exact.
+    ref = P.values(x, format).to(got.dtype).double()
+    assert torch.equal(got.double().cpu(), ref), f"{(got.double().cpu() != ref).sum()} of {ref.numel()} values differ"
+
+
+# ---------------------------------------------------------------- into four bits and back
+@pytest.mark.parametrize("format", FORMATS)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("rows,cols", [(1, 1), (1, 16), (3, 17), (5, 31), (2, 33), (129, 255), (7, 256), (4, 257), (131, 500), (33, 1000), (2, 2048),
+                                       (3, 2049), (5, 4097), (2, 8200), (3, 16384), (2, 16400), (1, 40001)])
+def test_values_are_the_nearest(format, dtype, rows, cols):
+    x = rows_like(rows, cols, rows * 1000 + cols, dtype)
+    q = ops().fp4_quantize(x.to(DEV), format)
+    same_values(x, format, ops().fp4_dequantize(q))
+    same_values(x, format, ops().fp4_dequantize(q, torch.bfloat16))
+
+
+@pytest.mark.parametrize("format", FORMATS)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_halves_go_to_the_even_code_under_every_scale(format, dtype):
+    """Values at, just below and just above every border, under all the scales that the format's blocks can have."""
+    borders = torch.tensor([.25, .75, 1.25, 1.75, 2.5, 3.5, 5], dtype=torch.float64)
+    b, blocks = P.BLOCK[format], []
+    step = 2.0 ** -7 if dtype == torch.bfloat16 else 2.0 ** -22
+    for e in range(-4, 5):
+        for m in range(8, 16):
+            s = m / 8 * 2.0 ** e if format == "nvfp4" else 2.0 ** e
+            near = torch.cat([borders * s * f for f in (1, 1 - step, 1 + step, 1 - 2 * step, 1 + 2 * step)])
+            block = torch.zeros(2 * b, dtype=torch.float64)
+            block[1:b] = near[:b - 1]
+            block[b + 1:2 * b] = near.flip(0)[:b - 1]
+            block[0] = block[b] = 6 * s
+            blocks.append(block * (-1 if m % 2 else 1))
+    x = torch.cat(blocks)[None].to(dtype)
+    x = torch.cat([x, -x, x * 2.0 ** -40, x * 2.0 ** 60])
+    same_values(x, format, ops().fp4_dequantize(ops().fp4_quantize(x.to(DEV), format)))
+
+
+@pytest.mark.parametrize("format", FORMATS)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_zeros_and_the_ends_of_the_range(format, dtype):
+    top = torch.finfo(dtype).max
+    x = torch.zeros(8, 96, dtype=dtype)
+    x[1, 5] = top
+    x[2, :48] = torch.finfo(dtype).tiny
+    x[3, 7], x[3, 40] = 2.0 ** -133, -2.0 ** -130          # below the normal numbers
+    x[4, 0], x[4, 50], x[4, 51], x[4, 90] = 1.0, 2.0 ** -14, 2.0 ** -18, 2.0 ** -30   # blocks far below the row's largest
+    x[5] = -0.0
+    x[6, 0], x[6, 20], x[6, 95] = -top, 1.0, 2.0 ** 100
+    x[7] = torch.linspace(-3, 3, 96)
+    same_values(x, format, ops().fp4_dequantize(ops().fp4_quantize(x.to(DEV), format)))
+
+
+@pytest.mark.parametrize("format", FORMATS)
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
+def test_a_row_that_is_not_finite_is_nan_and_the_others_are_as_ever(format, bad):
+    o, x, w = ops(), rows_like(5, 300, 1), rows_like(140, 300, 2)
+    x[2, 299] = bad
+    w[130, 0] = bad
+    qx, qw = o.fp4_quantize(x.to(DEV), format), o.fp4_quantize(w.to(DEV), format)
+    got = o.fp4_dequantize(qx).cpu()
+    assert got[2].isnan().all()
+    keep = [0, 1, 3, 4]
+    same_values(x[keep], format, got[keep])
+    y = o.fp4_gemm(qx, qw).cpu()
+    o.check_tc_status()
+    assert y[2].isnan().all() and y[:, 130].isnan().all()
+    others = [i for i in range(140) if i != 130]
+    assert y[keep][:, others].isfinite().all()
+
+
+@pytest.mark.parametrize("format", FORMATS)
+def test_rows_cut_out_of_wider_ones_and_a_matrix_filled_again(format):
+    o = ops()
+    wide = rows_like(20, 400, 3).to(DEV)
+    for at, cols in ((0, 200), (8, 200), (3, 129), (1, 320)):
+        x = wide[::2, at:at + cols]
+        same_values(x.cpu(), format, o.fp4_dequantize(o.fp4_quantize(x, format)))
+    q = o.fp4_quantize(wide, format)
+    again = rows_like(20, 400, 4).to(DEV)
+    assert o.fp4_quantize(again, format, out=q) is q
+    out = torch.full((40, 500), 7.0, device=DEV)
+    o.fp4_dequantize(q, out=out[::2, 10:410])
+    same_values(again.cpu(), format, out[::2, 10:410])
+    assert (out[1::2] == 7).all() and (out[:, :10] == 7).all() and (out[:, 410:] == 7).all()
+    one = wide[:1].expand(5, 400)                              # a row stride of 0
+    same_values(one.cpu(), format, o.fp4_dequantize(o.fp4_quantize(one, format)))
+
+
+@pytest.mark.parametrize("format", FORMATS)
+def test_codes_and_scales_lie_where_they_are_said_to(format):
+    x = rows_like(300, 700, 5)
+    q = ops().fp4_quantize(x.to(DEV), format)
+    code, scale, row = P.quantize(x, format)
+    got = q.codes.cpu()
+    assert got.shape == (300, 352)
+    low, high = (got & 15).long(), (got >> 4).long()
+    nibbles = torch.stack([low, high], 2).reshape(300, -1)
+    kinds = torch.cat([P.KINDS, -P.KINDS])
+    assert torch.equal(kinds[nibbles][:, :700], code.reshape(300, -1)[:, :700]) and (nibbles[:, 700:] & 7 == 0).all()
+    tiles = q.scales.cpu().view(3, -1, 32, 4, 4)                # row tile, four blocks, row % 32, row / 32, block
+    by_row = tiles.permute(0, 3, 2, 1, 4).reshape(384, -1)[:300].long()
+    e = (by_row - 127).double()
+    decoded = torch.pow(2.0, e) if format == "mxfp4" else by_row.to(torch.uint8).view(torch.float8_e4m3fn).double()
+    n = scale.shape[1]
+    assert torch.equal(decoded[:, :n], scale[:, :, 0]) and (by_row[:, n:] == 0).all()
+    assert torch.equal(q.row_scale.cpu().double(), row[:, 0])
+
+
+# ---------------------------------------------------------------- the product
+def check_product(M, N, K, format, out_dtype, seed, x=None, w=None):
+    """A term is exact in 32 bits; a sum of K terms in 32 bits is off by at most K 2^-23 of the sum of magnitudes, one truncation a term, whatever
+    its order, and a result in bfloat16 by half a step of its own, 2^-9 2 = 2^-8."""
+    o = ops()
+    x = rows_like(M, K, seed) if x is None else x
+    w = (rows_like(N, K, seed + 1, spread=2) * 0.02).to(torch.bfloat16) if w is None else w
+    got = o.fp4_gemm(o.fp4_quantize(x.to(DEV), format), o.fp4_quantize(w.to(DEV), format), out_dtype=out_dtype).double().cpu()
+    o.check_tc_status()
+    a, b = P.values(x, format), P.values(w, format)
+    ref, size = a @ b.T, a.abs() @ b.abs().T
+    tol = size * K * 2.0 ** -23 + (ref.abs() * 2.0 ** -8 if out_dtype == torch.bfloat16 else 0)
+    assert got.shape == (M, N)
+    far = (got - ref).abs() - tol
+    assert (far <= 0).all(), f"{int((far > 0).sum())} of {far.numel()} off, worst {float(far.max()):.3e} of {float(ref.abs().max()):.3e}"
+    return float((got - ref).norm() / ref.norm())
+
+
+@pytest.mark.parametrize("format", FORMATS)
+@pytest.mark.parametrize("M,N,K", [(1, 1, 1), (1, 128, 64), (1, 130, 256), (3, 7, 100), (8, 300, 512), (16, 128, 257), (17, 129, 300), (32, 500, 1024),
+                                   (33, 64, 96), (64, 256, 2048), (65, 127, 1500), (128, 384, 511), (129, 200, 768), (192, 128, 256), (193, 300, 400),
+                                   (320, 129, 1280), (385, 1000, 640), (700, 513, 300)])
+def test_product(format, M, N, K):
+    check_product(M, N, K, format, torch.float32, M + N + K)
+    check_product(M, N, K, format, torch.bfloat16, M + N + K)
+
+
+@pytest.mark.parametrize("format", FORMATS)
+def test_product_of_whole_numbers_is_exact(format):
+    """Codes and scales chosen so that every sum is a whole number below 2^24: any misplaced code, block scale or row scale shows."""
+    g = torch.Generator().manual_seed(9)
+    M, N, K = 200, 260, 640
+    b = P.BLOCK[format]
+
+    def matrix(rows):
+        code = torch.tensor([0., 1, 2, 3, 4, 6])[torch.randint(0, 6, (rows, K // b, b), generator=g)]
+        code[:, :, 0] = 6                                    # the block's scale is then the power of two beside it
+        sign = torch.where(torch.rand(rows, K // b, b, generator=g) < 0.5, -1.0, 1.0)
+        return (code * sign * torch.exp2(torch.randint(0, 3, (rows, K // b, 1), generator=g).float())).reshape(rows, K)
+    x, w = matrix(M), matrix(N)
+    o = ops()
+    qx, qw = o.fp4_quantize(x.to(DEV), format), o.fp4_quantize(w.to(DEV), format)
+    assert torch.equal(o.fp4_dequantize(qx).cpu(), x) and torch.equal(o.fp4_dequantize(qw).cpu(), w)
+    assert torch.equal(o.fp4_gemm(qx, qw).cpu().double(), x.double() @ w.double().T)
+    o.check_tc_status()
+
+
+@pytest.mark.parametrize("format", FORMATS)
+def test_product_into_rows_of_a_wider_result(format):
+    o = ops()
+    x, w = rows_like(37, 300, 1), rows_like(150, 300, 2)
+    qx, qw = o.fp4_quantize(x.to(DEV), format), o.fp4_quantize(w.to(DEV), format)
+    want = o.fp4_gemm(qx, qw)
+    out = torch.full((74, 200), 3.0, device=DEV)
+    o.fp4_gemm(qx, qw, out=out[::2, 7:157])
+    assert torch.equal(out[::2, 7:157], want)
+    assert (out[1::2] == 3).all() and (out[:, :7] == 3).all() and (out[:, 157:] == 3).all()
+
+
+@pytest.mark.parametrize("format", FORMATS)
+def test_a_tokens_result_does_not_hang_on_the_others(format):
+    o = ops()
+    x, w = rows_like(250, 700, 1).to(DEV), rows_like(300, 700, 2).to(DEV)
+    qw = o.fp4_quantize(w, format)
+    whole = o.fp4_gemm(o.fp4_quantize(x, format), qw)
+    for n in (1, 5, 16, 20, 40, 100, 128, 129, 200):
+        assert torch.equal(o.fp4_gemm(o.fp4_quantize(x[:n], format), qw), whole[:n])
+
+
+def test_nothing_to_do():
+    o = ops()
+    none = o.fp4_quantize(torch.empty(0, 64, dtype=torch.bfloat16, device=DEV))
+    some = o.fp4_quantize(rows_like(4, 64, 1).to(DEV))
+    assert o.fp4_dequantize(none).shape == (0, 64) and none.codes.shape == (0, 32)
+    assert o.fp4_gemm(none, some).shape == (0, 4) and o.fp4_gemm(some, none).shape == (4, 0)
+
+
+def test_on_another_stream_and_captured():
+    """The whole chain in a graph, replayed with other rows, on a stream of its own."""
+    o = ops()
+    x, w = rows_like(6, 512, 1).to(DEV), rows_like(400, 512, 2).to(DEV)
+    other = rows_like(6, 512, 3).to(DEV)
+    qw = o.fp4_quantize(w)
+    want, want2 = o.fp4_gemm(o.fp4_quantize(x), qw), o.fp4_gemm(o.fp4_quantize(other), qw)
+    q, out, held = o.Fp4Matrix(6, 512, "nvfp4", DEV), torch.empty(6, 400, device=DEV), x.clone()
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        o.fp4_gemm(o.fp4_quantize(held, out=q), qw, out=out)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=s):
+            o.fp4_gemm(o.fp4_quantize(held, out=q), qw, out=out)
+        s.synchronize()
+        out.zero_()
+        graph.replay()
+        s.synchronize()
+        assert torch.equal(out, want)
+        held.copy_(other)
+        graph.replay()
+        s.synchronize()
+        assert torch.equal(out, want2)
+
+
+def test_products_behind_products_read_what_the_last_one_left():
+    """Quantisation, product, quantisation of the result, product: every kernel starts while the one before it drains."""
+    o = ops()
+    x, w = rows_like(20, 256, 1).to(DEV), (rows_like(256, 256, 2, spread=1) * 0.1).to(DEV)
+    for format in FORMATS:
+        y = x
+        for _ in range(4):
+            qw = o.fp4_quantize(w, format)
+            z = o.fp4_gemm(o.fp4_quantize(y, format), qw, out_dtype=torch.bfloat16)
+            torch.cuda.synchronize()
+            again = o.fp4_gemm(o.fp4_quantize(y, format), qw, out_dtype=torch.bfloat16)
+            torch.cuda.synchronize()
+            assert torch.equal(z, again)
+            y = z
+        fast = x
+        for _ in range(4):
+            fast = o.fp4_gemm(o.fp4_quantize(fast, format), o.fp4_quantize(w, format), out_dtype=torch.bfloat16)
+        assert torch.equal(fast, y)

@@ -1,0 +1,98 @@
+"""What the operators of a step's output end refuse, told before anything is launched: on the CPU, where nothing could be."""
+import pytest
+import torch
+
+from libllm_b200.csrc import ops
+from libllm_b200.errors import ExtensionError, InvalidArgError, UnsupportedError
+
+I32 = torch.int32
+
+
+def matrix(rows, cols, format="nvfp4"):
+    return ops.Fp4Matrix(rows, cols, format, "cpu")
+
+
+@pytest.mark.parametrize("call", [
+    lambda: ops.Fp4Matrix(4, 0, "nvfp4", "cpu"),
+    lambda: ops.Fp4Matrix(-1, 4, "nvfp4", "cpu"),
+    lambda: ops.Fp4Matrix(4, 64, "fp4", "cpu"),
+    lambda: ops.fp4_quantize(torch.zeros(4, 64), "e2m1"),
+    lambda: ops.fp4_quantize(torch.zeros(64)),
+    lambda: ops.fp4_quantize(torch.zeros(64, 4).T),
+    lambda: ops.fp4_quantize(torch.zeros(4, 64), "nvfp4", out=matrix(4, 63)),
+    lambda: ops.fp4_quantize(torch.zeros(4, 64), "nvfp4", out=matrix(4, 64, "mxfp4")),
+    lambda: ops.fp4_dequantize(matrix(4, 64), out=torch.zeros(4, 63)),
+    lambda: ops.fp4_dequantize(matrix(4, 64), out=torch.zeros(1, 64).expand(4, 64)),
+    lambda: ops.fp4_gemm(matrix(4, 64), matrix(4, 65)),
+    lambda: ops.fp4_gemm(matrix(4, 64), matrix(4, 64, "mxfp4")),
+    lambda: ops.fp4_gemm(matrix(4, 64), matrix(5, 64), out=torch.zeros(5, 4)),
+    lambda: ops.fp4_gemm(matrix(4, 64), matrix(5, 64), out=torch.zeros(5, 4).T),
+    lambda: ops.fp4_gemm(matrix(4, 64), matrix(5, 64), out=torch.zeros(1, 5).expand(4, 5)),
+])
+def test_matrices_in_four_bits(call):
+    with pytest.raises(InvalidArgError):
+        call()
+
+
+@pytest.mark.parametrize("call", [
+    lambda: ops.fp4_quantize(torch.zeros(4, 64, dtype=torch.float16)),
+    lambda: ops.fp4_dequantize(matrix(4, 64), torch.float64),
+    lambda: ops.fp4_gemm(matrix(4, 64), matrix(5, 64), out_dtype=torch.float16),
+    lambda: ops.adjust_logits(torch.zeros(1, 5).expand(70000, 5)),
+])
+def test_types_and_sizes_that_are_not_taken(call):
+    with pytest.raises(UnsupportedError):
+        call()
+
+
+@pytest.mark.parametrize("call", [
+    lambda: ops.fp4_quantize(torch.zeros(4, 64)),
+    lambda: ops.fp4_dequantize(matrix(4, 64)),
+    lambda: ops.fp4_gemm(matrix(4, 64), matrix(5, 64)),
+    lambda: ops.adjust_logits(torch.zeros(4, 64)),
+])
+def test_there_is_no_way_to_run_without_a_device(call):
+    with pytest.raises(ExtensionError):
+        call()
+
+
+B, V = 3, 100
+HISTORY, LENGTHS = torch.zeros(5, 20, dtype=I32), torch.zeros(B, dtype=I32)
+
+
+@pytest.mark.parametrize("kw", [
+    dict(logits=torch.zeros(B, V, dtype=torch.bfloat16)),
+    dict(logits=torch.zeros(V)),
+    dict(logits=torch.zeros(V, B).T),
+    dict(out=torch.zeros(B, V + 1)),
+    dict(out=torch.zeros(B, V, dtype=torch.bfloat16)),
+    dict(out=torch.zeros(1, V).expand(B, V)),
+    dict(history=HISTORY),
+    dict(history=HISTORY.long(), lengths=LENGTHS),
+    dict(history=HISTORY[0], lengths=LENGTHS),
+    dict(history=HISTORY.T, lengths=LENGTHS),
+    dict(history=HISTORY[:2], lengths=LENGTHS),
+    dict(history=HISTORY, lengths=LENGTHS[:2]),
+    dict(history=HISTORY, lengths=LENGTHS.long()),
+    dict(history=HISTORY, lengths=LENGTHS, slots=LENGTHS.long()),
+    dict(history=HISTORY, lengths=LENGTHS, slots=LENGTHS[:1]),
+    dict(repetition=0.0),
+    dict(repetition=-1.0),
+    dict(repetition=float("inf")),
+    dict(presence=float("nan")),
+    dict(frequency=torch.zeros(B + 1)),
+    dict(frequency=torch.zeros(B, dtype=torch.float64)),
+    dict(bias=torch.zeros(V + 1)),
+    dict(bias=torch.zeros(1, V)),
+    dict(bias=torch.zeros(V, dtype=torch.bfloat16)),
+    dict(bias=torch.zeros(V, B).T),
+    dict(allowed=torch.zeros(3, dtype=I32)),
+    dict(allowed=torch.zeros(B, 5, dtype=I32)),
+    dict(allowed=torch.zeros(B, V, dtype=torch.bool)),
+    dict(allowed=torch.zeros(4, B, dtype=I32).T),
+])
+def test_logits_and_what_goes_with_them(kw):
+    kw = dict(kw)
+    logits = kw.pop("logits", torch.zeros(B, V))
+    with pytest.raises(InvalidArgError):
+        ops.adjust_logits(logits, **kw)
