@@ -56,8 +56,8 @@ FAMILIES: Dict[str, dict] = {
     "latent": dict(sources=["latent.cu"], headers=["common.cuh"]),
     "latent_tc": dict(sources=["latent_tc.cu"], headers=["common.cuh", "mma_tiles.cuh"]),
     "sampling": dict(sources=["sampling.cu"], headers=["common.cuh"]),
-    "logits": dict(sources=["logits.cu"], headers=["common.cuh"]),
-    "fp4": dict(sources=["fp4.cu"], headers=["common.cuh", "tc_common.cuh"]),
+    "logits": dict(sources=["logits.cu"], headers=["common.cuh", "logits.h"]),
+    "fp4": dict(sources=["fp4.cu"], headers=["common.cuh", "fp4.h", "tc_common.cuh"]),
     "moe": dict(sources=["moe.cu"], headers=["common.cuh", "mma_tiles.cuh"]),
     "moe_tc": dict(sources=["moe_tc.cu"], headers=["common.cuh", "tc_common.cuh"]),
     "gemv": dict(sources=["gemv.cu"], headers=["common.cuh"]),

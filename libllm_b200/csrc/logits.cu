@@ -8,12 +8,14 @@
 // history's ids of that slice in shared memory, and passes over its logits once.  Reading a history of thousands of ids once per slice
 // (from L2) costs less than 4 bytes of counts per token of the vocabulary from memory, and there is nothing to reset or to keep right.
 #include "common.cuh"
+#include "logits.h"
 
 LLM_DEFINE_LAST_ERROR(llm_logits_last_error)
 
 namespace {
 
-constexpr int AT = 512;                        // threads of a CTA
+constexpr int AT = 256;                        // threads of a CTA
+constexpr int MOST_SLICE = 4096;               // tokens of a CTA, at most: 16 KB of counters
 constexpr unsigned SEEN = 0x80000000u;         // a counter's highest bit: the token occurs; the others: how often it was drawn
 
 struct Rows {                                  // one number per row, or one for all
@@ -44,37 +46,80 @@ __device__ __forceinline__ float adjusted(float x, unsigned c, float rep, float 
   return n ? x - (freq * (float)n + pres) : x;
 }
 
+// The slice's ids among h[0 .. len).
+__device__ __forceinline__ void count(unsigned *counts, int id, int v0, int n) {
+  const unsigned at = (unsigned)(id < 0 ? ~id : id) - (unsigned)v0;
+  if (at < (unsigned)n) {
+    if (id >= 0) atomicAdd(&counts[at], 1u);             // any count but 0 says that the token occurs
+    else if (!(counts[at] & SEEN)) atomicOr(&counts[at], SEEN);
+  }
+}
+
 template <bool VEC>
 __global__ void __launch_bounds__(AT) adjust_kernel(Adjust a) {
-  extern __shared__ unsigned counts[];
+  extern __shared__ __align__(16) unsigned counts[];
   grid_dependents_launch();
   const long long b = blockIdx.y;
   const int v0 = blockIdx.x * a.slice, n = min(a.slice, a.V - v0);
   if (a.history)
-    for (int i = threadIdx.x; i < n; i += AT) counts[i] = 0;
+    for (int i = threadIdx.x * 4; i < n; i += AT * 4) *reinterpret_cast<uint4 *>(counts + i) = make_uint4(0, 0, 0, 0);
   grid_dependency_wait();
+  const float *x = a.logits + b * a.ld + v0, *bias = a.bias ? a.bias + b * a.ld_bias + v0 : nullptr;
+  const unsigned *allowed = a.allowed ? a.allowed + b * a.ld_allowed : nullptr;
+  float *out = a.out + b * a.ldo + v0;
+  // The slice's logits are on their way while the history is counted.
+  const int place = !a.history ? -1 : a.slots ? a.slots[b] : (int)b;
+  const int said = a.history ? a.lengths[b] : 0;
+  constexpr int AHEAD = MOST_SLICE / AT / 4;
+  float4 held[AHEAD];
+  if (VEC) {
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j) {
+      const int i = (threadIdx.x + j * AT) * 4;
+      if (i + 4 <= n) held[j] = *reinterpret_cast<const float4 *>(x + i);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j) {
+      float *v = reinterpret_cast<float *>(&held[j]);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int i = threadIdx.x + (4 * j + k) * AT;
+        if (i < n) v[k] = x[i];
+      }
+    }
+  }
   float rep = 1.f, pres = 0.f, freq = 0.f;
   if (a.history) {
     rep = a.repetition.at(b);
     pres = a.presence.at(b);
     freq = a.frequency.at(b);
-    __syncthreads();
-    const int place = a.slots ? a.slots[b] : (int)b;
-    const int len = place >= 0 && place < a.places ? min(max(a.lengths[b], 0), a.longest) : 0;
+    const int len = place >= 0 && place < a.places ? min(max(said, 0), a.longest) : 0;
     const int *h = a.history + (long long)place * a.ldh;
-    for (int i = threadIdx.x; i < len; i += AT) {
-      const int id = h[i];
-      const unsigned at = (unsigned)(id < 0 ? ~id : id) - (unsigned)v0;
-      if (at < (unsigned)n) {
-        if (id >= 0) atomicAdd(&counts[at], 1u);       // below, any count but 0 says that the token occurs
-        else if (!(counts[at] & SEEN)) atomicOr(&counts[at], SEEN);
+    __syncthreads();
+    int done = 0;
+    if (((uintptr_t)h & 15) == 0) {
+      done = len & ~3;
+      for (int i = threadIdx.x * 4; i < done; i += AT * 8) {         // two loads on their way
+        const int4 p = *reinterpret_cast<const int4 *>(h + i);
+        const bool two = i + AT * 4 < done;
+        const int4 q = two ? *reinterpret_cast<const int4 *>(h + i + AT * 4) : p;
+        count(counts, p.x, v0, n);
+        count(counts, p.y, v0, n);
+        count(counts, p.z, v0, n);
+        count(counts, p.w, v0, n);
+        if (two) {
+          count(counts, q.x, v0, n);
+          count(counts, q.y, v0, n);
+          count(counts, q.z, v0, n);
+          count(counts, q.w, v0, n);
+        }
       }
     }
+#pragma unroll 4
+    for (int i = done + threadIdx.x; i < len; i += AT) count(counts, h[i], v0, n);
     __syncthreads();
   }
-  const float *x = a.logits + b * a.ld + v0, *bias = a.bias ? a.bias + b * a.ld_bias + v0 : nullptr;
-  const unsigned *allowed = a.allowed ? a.allowed + b * a.ld_allowed : nullptr;
-  float *out = a.out + b * a.ldo + v0;
   auto one = [&](int i, float v) {
     if (a.history) v = adjusted(v, counts[i], rep, pres, freq);
     if (bias) v += bias[i];
@@ -82,14 +127,19 @@ __global__ void __launch_bounds__(AT) adjust_kernel(Adjust a) {
     return v;
   };
   if (VEC) {                                   // slices are multiples of 32 tokens
-    for (int i = threadIdx.x * 4; i + 4 <= n; i += AT * 4) {
-      float4 v = *reinterpret_cast<const float4 *>(x + i);
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j) {
+      const int i = (threadIdx.x + j * AT) * 4;
+      if (i + 4 > n) break;
+      float4 v = held[j];
       if (a.history) {
         const uint4 c = *reinterpret_cast<const uint4 *>(counts + i);
-        v.x = adjusted(v.x, c.x, rep, pres, freq);
-        v.y = adjusted(v.y, c.y, rep, pres, freq);
-        v.z = adjusted(v.z, c.z, rep, pres, freq);
-        v.w = adjusted(v.w, c.w, rep, pres, freq);
+        if (c.x | c.y | c.z | c.w) {
+          v.x = adjusted(v.x, c.x, rep, pres, freq);
+          v.y = adjusted(v.y, c.y, rep, pres, freq);
+          v.z = adjusted(v.z, c.z, rep, pres, freq);
+          v.w = adjusted(v.w, c.w, rep, pres, freq);
+        }
       }
       if (bias) {
         const float4 w = *reinterpret_cast<const float4 *>(bias + i);
@@ -110,31 +160,39 @@ __global__ void __launch_bounds__(AT) adjust_kernel(Adjust a) {
     const int i = (n & ~3) + threadIdx.x;
     if (i < n) out[i] = one(i, x[i]);
   } else {
-    for (int i = threadIdx.x; i < n; i += AT) out[i] = one(i, x[i]);
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j) {
+      const float *v = reinterpret_cast<const float *>(&held[j]);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int i = threadIdx.x + (4 * j + k) * AT;
+        if (i < n) out[i] = one(i, v[k]);
+      }
+    }
   }
 }
 
 }  // namespace
 
-// out [B, V] = logits [B, V] with the rows' penalties, bias and mask applied; out may be logits.  Row strides in elements (words for
-// `allowed`); a row stride of 0 for bias or allowed: one row for all.  repetition, presence, frequency: [B], or null and the number beside.
-LLM_EXPORT int llm_adjust_logits(const float *logits, long long ld, float *out, long long ldo, int B, int V, const int *history, long long ldh, int places,
-                                 int longest, const int *slots, const int *lengths, const float *repetition, float repetition_all, const float *presence,
-                                 float presence_all, const float *frequency, float frequency_all, const float *bias, long long ld_bias,
-                                 const int *allowed, long long ld_allowed, cudaStream_t stream) {
-  LLM_REQUIRE(B >= 0 && V >= 0, "adjust_logits: bad sizes %d x %d", B, V);
-  if (B == 0 || V == 0) return LLM_OK;
-  LLM_REQUIRE(B <= 65535, "adjust_logits: %d rows, at most 65535 are taken", B);
-  LLM_REQUIRE(!history || lengths, "adjust_logits: a history needs its rows' lengths");
-  LLM_REQUIRE(!history || slots || B <= places, "adjust_logits: %d rows, the history has %d", B, places);
-  Adjust a{logits, out, ld, ldo, V, 0, history, slots, lengths, ldh, places, longest, {repetition, repetition_all}, {presence, presence_all},
-           {frequency, frequency_all}, bias, ld_bias, (const unsigned *)allowed, ld_allowed};
-  int slice = 8192;
-  while (slice > 1024 && (long long)((V + slice - 1) / slice) * B < 4ll * sm_count()) slice /= 2;
+LLM_EXPORT int llm_adjust_logits(const AdjustLogitsCall *call) {
+  const AdjustLogitsCall &c = *call;
+  LLM_REQUIRE(c.B >= 0 && c.V >= 0 && c.V <= (1 << 30), "adjust_logits: bad sizes %lld x %lld", c.B, c.V);
+  if (c.B == 0 || c.V == 0) return LLM_OK;
+  LLM_REQUIRE(c.B <= 65535, "adjust_logits: %lld rows, at most 65535 are taken", c.B);
+  LLM_REQUIRE(!c.history || c.lengths, "adjust_logits: a history needs its rows' lengths");
+  LLM_REQUIRE(!c.history || (c.places > 0 && c.longest > 0 && c.places < (1ll << 31) && c.longest < (1ll << 31)),
+              "adjust_logits: a history of %lld places of %lld", c.places, c.longest);
+  LLM_REQUIRE(!c.history || c.slots || c.B <= c.places, "adjust_logits: %lld rows, the history has %lld places", c.B, c.places);
+  Adjust a{c.logits, c.out, c.ld, c.ldo, (int)c.V, 0, c.history, c.slots, c.lengths, c.ldh, (int)c.places, (int)c.longest,
+           {c.repetition, (float)c.repetition_all}, {c.presence, (float)c.presence_all}, {c.frequency, (float)c.frequency_all}, c.bias, c.ld_bias,
+           c.allowed, c.ld_allowed};
+  int slice = MOST_SLICE;
+  while (slice > 1024 && (c.V + slice - 1) / slice * c.B < 4ll * sm_count()) slice /= 2;
   a.slice = slice;
-  const bool vec = ((uintptr_t)logits | (uintptr_t)out | (uintptr_t)bias) % 16 == 0 && (ld | ldo | (bias ? ld_bias : 0)) % 4 == 0;
-  const dim3 grid((unsigned)((V + slice - 1) / slice), (unsigned)B);
-  const size_t smem = history ? (size_t)slice * sizeof(unsigned) : 0;
+  const bool vec = ((uintptr_t)c.logits | (uintptr_t)c.out | (uintptr_t)c.bias) % 16 == 0 && (c.ld | c.ldo | (c.bias ? c.ld_bias : 0)) % 4 == 0;
+  const dim3 grid((unsigned)((c.V + slice - 1) / slice), (unsigned)c.B);
+  const size_t smem = c.history ? (size_t)slice * sizeof(unsigned) : 0;
+  const cudaStream_t stream = (cudaStream_t)c.stream;
   LLM_CHECK_CUDA(vec ? llm_launch(adjust_kernel<true>, grid, dim3(AT), smem, stream, a) : llm_launch(adjust_kernel<false>, grid, dim3(AT), smem, stream, a),
                  "adjust_logits launch");
   return LLM_OK;

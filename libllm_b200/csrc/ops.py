@@ -6,7 +6,8 @@ from __future__ import annotations
 
 import ctypes
 import math
-from ctypes import c_float, c_int, c_longlong, c_void_p
+import struct
+from ctypes import c_char_p, c_float, c_int, c_longlong, c_void_p
 from typing import Optional
 
 import torch
@@ -70,10 +71,29 @@ def _call(family: str, name: str, argtypes, *args) -> None:
     LAUNCHES[0] += 1
     status = f(*args)
     if status != 0:
-        msg = err().decode("utf-8", "replace")
-        if status == 0x0100:
-            raise UnsupportedError(msg)
-        raise ExtensionError(f"{name} failed (status {status:#x}): {msg}")
+        _raise(name, status, err)
+
+
+_packed = {}
+
+
+def _call_packed(family: str, name: str, args: bytes) -> None:
+    """A function that takes its arguments as one struct of 64-bit fields.  A dozen arguments converted one by one cost more than
+    the launch itself."""
+    f = _packed.get(name)
+    if f is None:
+        f = _packed[name] = _fn(family, name, [c_char_p])
+    LAUNCHES[0] += 1
+    status = f[0](args)
+    if status != 0:
+        _raise(name, status, f[1])
+
+
+def _raise(name: str, status: int, err) -> None:
+    msg = err().decode("utf-8", "replace")
+    if status == 0x0100:
+        raise UnsupportedError(msg)
+    raise ExtensionError(f"{name} failed (status {status:#x}): {msg}")
 
 
 # ------------------------------------------------------------------ elementwise
@@ -341,13 +361,20 @@ def sample(logits: torch.Tensor, temperature: float, top_k: int, top_p: float, u
     return out
 
 
-def _same_device(*tensors) -> None:
-    """The tensors lie on the current device, where the launch goes."""
-    _on_gpu(*tensors)
+def _same_device(*tensors) -> int:
+    """The tensors lie on the current device, where the launch goes; its current stream's handle."""
+    if not tensors[0].is_cuda:
+        _on_gpu(tensors[0])
     current = torch.cuda.current_device()
     for t in tensors:
-        if t is not None and t.device.index != current:
+        if t is not None and t.get_device() != current:
+            _on_gpu(t)
             raise InvalidArgError(f"a tensor lies on '{t.device}', the launch goes to the current device 'cuda:{current}'")
+    return _raw_stream(current) if _raw_stream is not None else torch.cuda.current_stream().cuda_stream
+
+
+def _address(t: Optional[torch.Tensor]) -> int:
+    return 0 if t is None else t.data_ptr()
 
 
 def _per_row(name: str, v, rows: int, *, positive: bool = False):
@@ -362,8 +389,7 @@ def _per_row(name: str, v, rows: int, *, positive: bool = False):
     return None, v
 
 
-_ADJUST_ARGS = [c_void_p, c_longlong, c_void_p, c_longlong, c_int, c_int, c_void_p, c_longlong, c_int, c_int, c_void_p, c_void_p, c_void_p, c_float,
-                c_void_p, c_float, c_void_p, c_float, c_void_p, c_longlong, c_void_p, c_longlong, c_void_p]
+_pack_adjust = struct.Struct("@PqPqqqPqqqPPPPPdddPqPqP").pack            # csrc/logits.h: AdjustLogitsCall
 
 
 def adjust_logits(logits: torch.Tensor, out: Optional[torch.Tensor] = None, history: Optional[torch.Tensor] = None,
@@ -399,9 +425,9 @@ def adjust_logits(logits: torch.Tensor, out: Optional[torch.Tensor] = None, hist
                 raise InvalidArgError(f"adjust_logits: {name} are contiguous int32 with one per row ({B})")
         if places * longest == 0:
             history = None                      # nothing was said
-    repetition, rep_all = _per_row("repetition", repetition, B, positive=True)
-    presence, pres_all = _per_row("presence", presence, B)
-    frequency, freq_all = _per_row("frequency", frequency, B)
+    rep, rep_all = _per_row("repetition", repetition, B, positive=True)
+    pres, pres_all = _per_row("presence", presence, B)
+    freq, freq_all = _per_row("frequency", frequency, B)
     ldb = lda = 0
     if bias is not None:
         if bias.dtype != torch.float32 or bias.shape not in ((V,), (B, V)) or (V > 1 and bias.stride(-1) != 1):
@@ -412,12 +438,12 @@ def adjust_logits(logits: torch.Tensor, out: Optional[torch.Tensor] = None, hist
         if allowed.dtype != torch.int32 or allowed.shape not in ((words,), (B, words)) or (words > 1 and allowed.stride(-1) != 1):
             raise InvalidArgError(f"adjust_logits: allowed is int32 [{words}] or [{B}, {words}] (a bit per token) with neighbouring words")
         lda = allowed.stride(0) if allowed.dim() == 2 else 0
-    _same_device(logits, out, history, slots, lengths, repetition, presence, frequency, bias, allowed)
+    stream = _same_device(logits, out, history, slots, lengths, rep, pres, freq, bias, allowed)
     if out is None:
         out = torch.empty(B, V, dtype=torch.float32, device=logits.device)
-    _call("logits", "llm_adjust_logits", _ADJUST_ARGS, _ptr(logits), logits.stride(0), _ptr(out), out.stride(0), B, V, _ptr(history), ldh, places, longest,
-          _ptr(slots), _ptr(lengths), _ptr(repetition), rep_all, _ptr(presence), pres_all, _ptr(frequency), freq_all, _ptr(bias), ldb, _ptr(allowed),
-          lda, _stream())
+    _call_packed("logits", "llm_adjust_logits", _pack_adjust(
+        logits.data_ptr(), logits.stride(0), out.data_ptr(), out.stride(0), B, V, _address(history), ldh, places, longest, _address(slots), _address(lengths),
+        _address(rep), _address(pres), _address(freq), rep_all, pres_all, freq_all, _address(bias), ldb, _address(allowed), lda, stream))
     return out
 
 
@@ -425,22 +451,33 @@ def adjust_logits(logits: torch.Tensor, out: Optional[torch.Tensor] = None, hist
 FP4_FORMATS = {"nvfp4": 0, "mxfp4": 1}
 
 
+_fp4_layouts = {}
+
+
+def _fp4_layout(rows: int, cols: int, format: str):
+    """(format's number, where codes end, where scales begin, where the row scales begin, where they end) in the bytes of a matrix."""
+    if format not in FP4_FORMATS:
+        raise InvalidArgError(f"fp4: format '{format}' is not known ({' or '.join(FP4_FORMATS)})")
+    if rows < 0 or not 0 < cols <= 1 << 28:
+        raise InvalidArgError(f"fp4: a matrix of {rows} x {cols} is not taken")
+    codes = rows * ((cols + 31) // 32 * 16)
+    at = (codes + 511) // 512 * 512
+    end = at + (rows + 127) // 128 * ((cols + 255) // 256) * (2048 if format == "nvfp4" else 1024)
+    if len(_fp4_layouts) > 4096:
+        _fp4_layouts.clear()
+    layout = _fp4_layouts[rows, cols, format] = (FP4_FORMATS[format], codes, at, end, end + 4 * rows)
+    return layout
+
+
 class Fp4Matrix:
     """A matrix [rows, cols] in four bits (csrc/fp4.cu says what lies where): codes, block scales and row scales in one piece of device
     memory.  ``fp4_quantize`` makes one or fills one again."""
-    __slots__ = ("rows", "cols", "format", "data", "_at")
+    __slots__ = ("rows", "cols", "format", "data", "_layout")
 
-    def __init__(self, rows: int, cols: int, format: str = "nvfp4", device=None):
-        if format not in FP4_FORMATS:
-            raise InvalidArgError(f"fp4: format '{format}' is not known ({' or '.join(FP4_FORMATS)})")
-        if rows < 0 or not 0 < cols <= 1 << 28:
-            raise InvalidArgError(f"fp4: a matrix of {rows} x {cols} is not taken")
+    def __init__(self, rows: int, cols: int, format: str = "nvfp4", device="cuda"):
+        self._layout = _fp4_layouts.get((rows, cols, format)) or _fp4_layout(rows, cols, format)
         self.rows, self.cols, self.format = rows, cols, format
-        codes = rows * ((cols + 31) // 32 * 16)
-        scales = (rows + 127) // 128 * ((cols + 255) // 256) * (2048 if format == "nvfp4" else 1024)
-        at = (codes + 511) // 512 * 512
-        self._at = (codes, at, at + scales, at + scales + 4 * rows)
-        self.data = torch.empty(max(self._at[3], 1), dtype=torch.uint8, device="cuda" if device is None else device)
+        self.data = torch.empty(self._layout[4], dtype=torch.uint8, device=device)
 
     @property
     def device(self):
@@ -448,30 +485,35 @@ class Fp4Matrix:
 
     @property
     def nbytes(self) -> int:
-        return self._at[3]
+        return self._layout[4]
 
     @property
     def codes(self) -> torch.Tensor:
         """uint8 [rows, bytes of a row]: two codes a byte, the lower four bits first."""
-        return self.data[:self._at[0]].view(self.rows, -1) if self.rows else self.data.new_empty(0, (self.cols + 31) // 32 * 16)
+        return self.data[:self._layout[1]].view(self.rows, (self.cols + 31) // 32 * 16)
 
     @property
     def scales(self) -> torch.Tensor:
         """uint8, tiles of 128 rows x 4 blocks."""
-        return self.data[self._at[1]:self._at[2]]
+        return self.data[self._layout[2]:self._layout[3]]
 
     @property
     def row_scale(self) -> torch.Tensor:
-        return self.data[self._at[2]:self._at[3]].view(torch.float32)
-
-    def _pointers(self):
-        p = self.data.data_ptr()
-        return c_void_p(p), c_void_p(p + self._at[1]), c_void_p(p + self._at[2])
+        return self.data[self._layout[3]:].view(torch.float32)
 
 
-_FP4_QUANTIZE_ARGS = [c_int, c_void_p, c_longlong, c_void_p, c_void_p, c_void_p, c_longlong, c_int, c_int, c_void_p]
-_FP4_DEQUANTIZE_ARGS = [c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_longlong, c_longlong, c_int, c_int, c_void_p]
-_FP4_GEMM_ARGS = [c_void_p] * 6 + [c_int, c_void_p, c_longlong, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p]
+# csrc/fp4.h: Fp4QuantizeCall, Fp4DequantizeCall, Fp4GemmCall
+_pack_fp4_quantize, _pack_fp4_dequantize = struct.Struct("@qPqPPPqqqP").pack, struct.Struct("@PPPqPqqqqP").pack
+_pack_fp4_gemm = struct.Struct("@PPPPPPqPqqqqqqPP").pack
+_status_words = {}
+
+
+def _status_word(device) -> int:
+    """tc_status' address."""
+    p = _status_words.get(device.index)
+    if p is None:
+        p = _status_words[device.index] = tc_status(device).data_ptr()
+    return p
 
 
 def fp4_quantize(x: torch.Tensor, format: str = "nvfp4", out: Optional[Fp4Matrix] = None) -> Fp4Matrix:
@@ -482,14 +524,18 @@ def fp4_quantize(x: torch.Tensor, format: str = "nvfp4", out: Optional[Fp4Matrix
         raise InvalidArgError("fp4_quantize: x is [rows, cols] with neighbouring columns")
     dt = dtype_code(x.dtype)
     rows, cols = x.shape
-    if format not in FP4_FORMATS:
-        raise InvalidArgError(f"fp4_quantize: format '{format}' is not known ({' or '.join(FP4_FORMATS)})")
-    if out is not None and (out.rows, out.cols, out.format) != (rows, cols, format):
-        raise InvalidArgError(f"fp4_quantize: out is {out.format} [{out.rows}, {out.cols}], x becomes {format} [{rows}, {cols}]")
-    _same_device(x, out.data if out is not None else None)
     if out is None:
+        if (rows, cols, format) not in _fp4_layouts:
+            _fp4_layout(rows, cols, format)
+        stream = _same_device(x)
         out = Fp4Matrix(rows, cols, format, x.device)
-    _call("fp4", "llm_fp4_quantize", _FP4_QUANTIZE_ARGS, dt, _ptr(x), x.stride(0), *out._pointers(), rows, cols, FP4_FORMATS[format], _stream())
+    else:
+        if (out.rows, out.cols, out.format) != (rows, cols, format):
+            raise InvalidArgError(f"fp4_quantize: out is {out.format} [{out.rows}, {out.cols}], x becomes {format} [{rows}, {cols}]")
+        stream = _same_device(x, out.data)
+    number, _, scales, row, _ = out._layout
+    p = out.data.data_ptr()
+    _call_packed("fp4", "llm_fp4_quantize", _pack_fp4_quantize(dt, x.data_ptr(), x.stride(0), p, p + scales, p + row, rows, cols, number, stream))
     return out
 
 
@@ -499,11 +545,12 @@ def fp4_dequantize(q: Fp4Matrix, dtype: torch.dtype = torch.float32, out: Option
     dt = dtype_code(dtype if out is None else out.dtype)
     if out is not None and (out.shape != (q.rows, q.cols) or (q.cols > 1 and out.stride(1) != 1) or (q.rows > 1 and out.stride(0) < q.cols)):
         raise InvalidArgError(f"fp4_dequantize: out is [{q.rows}, {q.cols}] with neighbouring columns and rows of its own")
-    _same_device(q.data, out)
+    stream = _same_device(q.data, out)
     if out is None:
-        out = torch.empty(q.rows, q.cols, dtype=dtype, device=q.device)
-    _call("fp4", "llm_fp4_dequantize", _FP4_DEQUANTIZE_ARGS, *q._pointers(), dt, _ptr(out), out.stride(0), q.rows, q.cols,
-          FP4_FORMATS[q.format], _stream())
+        out = torch.empty(q.rows, q.cols, dtype=dtype, device=q.data.device)
+    number, _, scales, row, _ = q._layout
+    p = q.data.data_ptr()
+    _call_packed("fp4", "llm_fp4_dequantize", _pack_fp4_dequantize(p, p + scales, p + row, dt, out.data_ptr(), out.stride(0), q.rows, q.cols, number, stream))
     return out
 
 
@@ -518,11 +565,14 @@ def fp4_gemm(x: Fp4Matrix, w: Fp4Matrix, out: Optional[torch.Tensor] = None, out
     dt = dtype_code(out_dtype if out is None else out.dtype)
     if out is not None and (out.shape != (M, N) or (N > 1 and out.stride(1) != 1) or (M > 1 and out.stride(0) < N)):
         raise InvalidArgError(f"fp4_gemm: out is [{M}, {N}] with neighbouring columns and rows of its own")
-    _same_device(x.data, w.data, out)
+    stream = _same_device(x.data, w.data, out)
     if out is None:
-        out = torch.empty(M, N, dtype=out_dtype, device=w.device)
-    _call("fp4", "llm_fp4_gemm", _FP4_GEMM_ARGS, *x._pointers(), *w._pointers(), dt, _ptr(out), out.stride(0), M, N, x.cols,
-          FP4_FORMATS[x.format], 0, _ptr(tc_status(w.device)), _stream())
+        out = torch.empty(M, N, dtype=out_dtype, device=w.data.device)
+    number, _, xs, xr, _ = x._layout
+    _, _, ws, wr, _ = w._layout
+    xp, wp = x.data.data_ptr(), w.data.data_ptr()
+    _call_packed("fp4", "llm_fp4_gemm", _pack_fp4_gemm(xp, xp + xs, xp + xr, wp, wp + ws, wp + wr, dt, out.data_ptr(), out.stride(0), M, N, x.cols, number, 0,
+                                                       _status_word(w.data.device), stream))
     return out
 
 

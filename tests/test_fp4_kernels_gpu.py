@@ -153,7 +153,7 @@ def check_product(M, N, K, format, out_dtype, seed, x=None, w=None):
 @pytest.mark.parametrize("format", FORMATS)
 @pytest.mark.parametrize("M,N,K", [(1, 1, 1), (1, 128, 64), (1, 130, 256), (3, 7, 100), (8, 300, 512), (16, 128, 257), (17, 129, 300), (32, 500, 1024),
                                    (33, 64, 96), (64, 256, 2048), (65, 127, 1500), (128, 384, 511), (129, 200, 768), (192, 128, 256), (193, 300, 400),
-                                   (320, 129, 1280), (385, 1000, 640), (700, 513, 300)])
+                                   (320, 129, 1280), (385, 1000, 640), (700, 513, 300), (256, 192, 256), (257, 193, 511), (1000, 1, 64), (511, 576, 2048), (1030, 2000, 500)])
 def test_product(format, M, N, K):
     check_product(M, N, K, format, torch.float32, M + N + K)
     check_product(M, N, K, format, torch.bfloat16, M + N + K)
@@ -180,15 +180,19 @@ def test_product_of_whole_numbers_is_exact(format):
 
 
 @pytest.mark.parametrize("format", FORMATS)
-def test_product_into_rows_of_a_wider_result(format):
+@pytest.mark.parametrize("M", [37, 300, 1100])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_product_into_rows_of_a_wider_result(format, M, dtype):
     o = ops()
-    x, w = rows_like(37, 300, 1), rows_like(150, 300, 2)
+    N = 250
+    x, w = rows_like(M, 300, 1), rows_like(N, 300, 2)
     qx, qw = o.fp4_quantize(x.to(DEV), format), o.fp4_quantize(w.to(DEV), format)
-    want = o.fp4_gemm(qx, qw)
-    out = torch.full((74, 200), 3.0, device=DEV)
-    o.fp4_gemm(qx, qw, out=out[::2, 7:157])
-    assert torch.equal(out[::2, 7:157], want)
-    assert (out[1::2] == 3).all() and (out[:, :7] == 3).all() and (out[:, 157:] == 3).all()
+    want = o.fp4_gemm(qx, qw, out_dtype=dtype)
+    for at, wide in ((7, 400), (8, 400), (8, 401), (0, 250)):             # rows on 16 bytes and not
+        out = torch.full((2 * M, wide), 3.0, device=DEV, dtype=dtype)
+        o.fp4_gemm(qx, qw, out=out[::2, at:at + N])
+        assert torch.equal(out[::2, at:at + N], want)
+        assert (out[1::2] == 3).all() and (out[:, :at] == 3).all() and (out[:, at + N:] == 3).all()
 
 
 @pytest.mark.parametrize("format", FORMATS)
