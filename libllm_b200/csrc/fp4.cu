@@ -728,15 +728,16 @@ int get_code_map(const void *codes, long long rows, long long K, int box_rows, C
   return LLM_OK;
 }
 
-// Parts of K of a product of few tokens, from the sizes of the matrix alone so that a token's sums do not hang on how many others there are: as many as still
-// leave every CTA an SM of its own and every part two stages.
-int k_parts(int N, int K) {
+// Parts of K of a product of up to 128 tokens: as many as leave every CTA an SM of its own, eight only of matrices with 8 tiles or fewer (16
+// clusters of 8 CTAs are not on the chip at once).  Handing sums over costs more the more tokens there are: up to 32 tokens, two stages to a part are
+// enough; beyond, four parts or eight of 32 stages or more.  In 1 / 2 / 4 / 8 parts, us: 2,048 features, K = 2,048, 1 token 5.1 / 4.2 / 3.6 / 3.6, 64 tokens
+// 5.5 / 7.3 / 5.7 / 5.7; K = 1,024, 8 tokens 3.5 / 4.0; K = 8,192, 8 tokens 11.5 / 8.5 / 6.2 / 8.7, 64 tokens 11.9 / 10.9 / 8.0 / 12.3, 128 tokens 13.1 / 14.2 /
+// 10.7 / 17.1; 512 features, K = 16,384, 1 token 19.5 / 12.1 / 8.0 / 5.9; 8,192 features, K = 8,192, 8 tokens 11.9 / 10.4, 64 tokens 12.7 / 13.1.
+int k_parts(int M, int N, int K) {
   const long long tiles = (N + FP_ROWS - 1) / FP_ROWS, stages = k_stages(K);
-  static const int most = getenv("FP4_PARTS") ? atoi(getenv("FP4_PARTS")) : 8;
-  static const int least = getenv("FP4_LEAST") ? atoi(getenv("FP4_LEAST")) : 2;
   int parts = 1;
-  while (parts < most && tiles * parts * 2 <= sm_count() && stages >= parts * 2 * least) parts *= 2;
-  return parts;
+  while (parts < 8 && tiles * parts * 2 <= (parts == 4 ? 64 : sm_count()) && stages >= 8 && stages >= parts * 4) parts *= 2;
+  return M <= 32 || (parts >= 4 && stages >= 32) ? parts : 1;
 }
 
 template <int TN, int FORMAT, typename TO>
@@ -1138,7 +1139,7 @@ int dispatch_fp4(const void *x_codes, const void *w_codes, const Fp4In &in, void
                  int *status, cudaStream_t stream) {
 #define FP4_GO(TN, PARTS) return launch_fp4<TN, FORMAT, TO>(x_codes, w_codes, in, out, ldo, M, N, K, PARTS, weights_first, status, stream)
   if (M <= 128) {
-    const int parts = k_parts(N, K);
+    const int parts = k_parts(M, N, K);
     if (M <= 16) FP4_GO(16, parts);
     if (M <= 32) FP4_GO(32, parts);
     if (M <= 64) FP4_GO(64, parts);

@@ -16,6 +16,7 @@ from ..errors import ExtensionError, InvalidArgError, UnsupportedError
 from . import build
 
 F32, BF16 = 0, 1
+_F32, _I32 = torch.float32, torch.int32
 _DT = {torch.float32: F32, torch.bfloat16: BF16}
 
 
@@ -361,32 +362,32 @@ def sample(logits: torch.Tensor, temperature: float, top_k: int, top_p: float, u
     return out
 
 
-def _same_device(*tensors) -> int:
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+
+
+def _same_device(first: torch.Tensor, *others) -> int:
     """The tensors lie on the current device, where the launch goes; its current stream's handle."""
-    if not tensors[0].is_cuda:
-        _on_gpu(tensors[0])
-    current = torch.cuda.current_device()
-    for t in tensors:
+    if not first.is_cuda:
+        _on_gpu(first)
+    current = _current_device()
+    for t in (first, *others):
         if t is not None and t.get_device() != current:
             _on_gpu(t)
             raise InvalidArgError(f"a tensor lies on '{t.device}', the launch goes to the current device 'cuda:{current}'")
     return _raw_stream(current) if _raw_stream is not None else torch.cuda.current_stream().cuda_stream
 
 
-def _address(t: Optional[torch.Tensor]) -> int:
-    return 0 if t is None else t.data_ptr()
-
-
 def _per_row(name: str, v, rows: int, *, positive: bool = False):
-    """A number for all rows, or a 32-bit tensor with one per row: (the tensor or None, the number)."""
-    if isinstance(v, torch.Tensor):
-        if v.dtype != torch.float32 or v.shape != (rows,) or not v.is_contiguous():
-            raise InvalidArgError(f"adjust_logits: {name} is a number or a contiguous float32 tensor with one per row ({rows})")
-        return v, 0.0
-    v = float(v)
+    """A number for all rows, or a 32-bit tensor with one per row: (the tensor or None, its address or 0, the number)."""
+    if type(v) is not float:
+        if isinstance(v, torch.Tensor):
+            if v.dtype != _F32 or v.dim() != 1 or v.size(0) != rows or not v.is_contiguous():
+                raise InvalidArgError(f"adjust_logits: {name} is a number or a contiguous float32 tensor with one per row ({rows})")
+            return v, v.data_ptr(), 0.0
+        v = float(v)
     if not math.isfinite(v) or (positive and v <= 0):
         raise InvalidArgError(f"adjust_logits: {name} must be a finite{' positive' if positive else ''} number, got {v}")
-    return None, v
+    return None, 0, v
 
 
 _pack_adjust = struct.Struct("@PqPqqqPqqqPPPPPdddPqPqP").pack            # csrc/logits.h: AdjustLogitsCall
@@ -404,46 +405,54 @@ def adjust_logits(logits: torch.Tensor, out: Optional[torch.Tensor] = None, hist
     itself without slots; a place outside the history: an empty one), an id for a token that was drawn, ~id for one that a prompt brought; ids
     outside the vocabulary count for nothing.  repetition (above 0), presence and frequency: a number, or a float32 tensor [B]; without a
     history they do nothing.  ``out`` (new where None) may be ``logits`` itself, and no other tensor that overlaps it.  All 32-bit."""
-    if logits.dim() != 2 or logits.dtype != torch.float32 or (logits.shape[1] > 1 and logits.stride(1) != 1):
-        raise InvalidArgError("adjust_logits: logits are float32 [rows, vocabulary] with neighbouring columns")
+    if logits.dim() != 2 or logits.dtype != _F32:
+        raise InvalidArgError("adjust_logits: logits are float32 [rows, vocabulary]")
     B, V = logits.shape
+    ld, ld1 = logits.stride()
+    if ld1 != 1 and V > 1:
+        raise InvalidArgError("adjust_logits: the logits of a row are neighbours")
     if B > 65535 or V > 1 << 30:
         raise UnsupportedError(f"adjust_logits: {B} rows of {V} logits are not taken")
-    if out is not None and (out.dtype != torch.float32 or out.shape != logits.shape or (V > 1 and out.stride(1) != 1) or (B > 1 and out.stride(0) < V)):
-        raise InvalidArgError("adjust_logits: out has the logits' shape and type, and rows of its own")
-    ldh = places = longest = 0
+    ldo = V
+    if out is not None:
+        ldo = out.stride(0) if out.dim() == 2 else 0
+        if out.dtype != _F32 or out.shape != logits.shape or (V > 1 and out.stride(1) != 1) or (B > 1 and ldo < V):
+            raise InvalidArgError("adjust_logits: out has the logits' shape and type, and rows of its own")
+    ph = ldh = places = longest = ps = pl = 0
     if history is not None:
-        if history.dim() != 2 or history.dtype != torch.int32 or (history.shape[1] > 1 and history.stride(1) != 1):
+        if history.dim() != 2 or history.dtype != _I32 or (history.stride(1) != 1 and history.size(1) > 1):
             raise InvalidArgError("adjust_logits: the history is int32 [places, longest] with neighbouring entries")
+        if lengths is None or lengths.dtype != _I32 or lengths.dim() != 1 or lengths.size(0) != B or not lengths.is_contiguous():
+            raise InvalidArgError(f"adjust_logits: lengths are contiguous int32 with one per row ({B})")
         places, longest = history.shape
-        ldh = history.stride(0)
-        for name, t in (("lengths", lengths), ("slots", slots)):
-            if t is None and name == "slots":
-                if B > places:
-                    raise InvalidArgError(f"adjust_logits: {B} rows without slots, the history has {places} places")
-            elif t is None or t.dtype != torch.int32 or t.shape != (B,) or not t.is_contiguous():
-                raise InvalidArgError(f"adjust_logits: {name} are contiguous int32 with one per row ({B})")
-        if places * longest == 0:
-            history = None                      # nothing was said
-    rep, rep_all = _per_row("repetition", repetition, B, positive=True)
-    pres, pres_all = _per_row("presence", presence, B)
-    freq, freq_all = _per_row("frequency", frequency, B)
-    ldb = lda = 0
+        if slots is not None:
+            if slots.dtype != _I32 or slots.dim() != 1 or slots.size(0) != B or not slots.is_contiguous():
+                raise InvalidArgError(f"adjust_logits: slots are contiguous int32 with one per row ({B})")
+            ps = slots.data_ptr()
+        elif B > places:
+            raise InvalidArgError(f"adjust_logits: {B} rows without slots, the history has {places} places")
+        if places * longest > 0:                # else nothing was said
+            ph, pl, ldh = history.data_ptr(), lengths.data_ptr(), history.stride(0)
+    rep, pr, rep_all = _per_row("repetition", repetition, B, positive=True)
+    pres, pp, pres_all = _per_row("presence", presence, B)
+    freq, pf, freq_all = _per_row("frequency", frequency, B)
+    pb = ldb = pa = lda = 0
     if bias is not None:
-        if bias.dtype != torch.float32 or bias.shape not in ((V,), (B, V)) or (V > 1 and bias.stride(-1) != 1):
+        n = bias.dim()
+        if bias.dtype != _F32 or not 1 <= n <= 2 or bias.size(n - 1) != V or (n == 2 and bias.size(0) != B) or (V > 1 and bias.stride(n - 1) != 1):
             raise InvalidArgError(f"adjust_logits: the bias is float32 [{V}] or [{B}, {V}] with neighbouring columns")
-        ldb = bias.stride(0) if bias.dim() == 2 else 0
+        pb, ldb = bias.data_ptr(), bias.stride(0) if n == 2 else 0
     if allowed is not None:
-        words = (V + 31) // 32
-        if allowed.dtype != torch.int32 or allowed.shape not in ((words,), (B, words)) or (words > 1 and allowed.stride(-1) != 1):
+        n, words = allowed.dim(), (V + 31) // 32
+        if (allowed.dtype != _I32 or not 1 <= n <= 2 or allowed.size(n - 1) != words or (n == 2 and allowed.size(0) != B)
+                or (words > 1 and allowed.stride(n - 1) != 1)):
             raise InvalidArgError(f"adjust_logits: allowed is int32 [{words}] or [{B}, {words}] (a bit per token) with neighbouring words")
-        lda = allowed.stride(0) if allowed.dim() == 2 else 0
+        pa, lda = allowed.data_ptr(), allowed.stride(0) if n == 2 else 0
     stream = _same_device(logits, out, history, slots, lengths, rep, pres, freq, bias, allowed)
     if out is None:
-        out = torch.empty(B, V, dtype=torch.float32, device=logits.device)
+        out = torch.empty(B, V, dtype=_F32, device=logits.device)
     _call_packed("logits", "llm_adjust_logits", _pack_adjust(
-        logits.data_ptr(), logits.stride(0), out.data_ptr(), out.stride(0), B, V, _address(history), ldh, places, longest, _address(slots), _address(lengths),
-        _address(rep), _address(pres), _address(freq), rep_all, pres_all, freq_all, _address(bias), ldb, _address(allowed), lda, stream))
+        logits.data_ptr(), ld, out.data_ptr(), ldo, B, V, ph, ldh, places, longest, ps, pl, pr, pp, pf, rep_all, pres_all, freq_all, pb, ldb, pa, lda, stream))
     return out
 
 
@@ -475,9 +484,11 @@ class Fp4Matrix:
     __slots__ = ("rows", "cols", "format", "data", "_layout")
 
     def __init__(self, rows: int, cols: int, format: str = "nvfp4", device="cuda"):
-        self._layout = _fp4_layouts.get((rows, cols, format)) or _fp4_layout(rows, cols, format)
-        self.rows, self.cols, self.format = rows, cols, format
-        self.data = torch.empty(self._layout[4], dtype=torch.uint8, device=device)
+        self._layout = layout = _fp4_layouts.get((rows, cols, format)) or _fp4_layout(rows, cols, format)
+        self.rows = rows
+        self.cols = cols
+        self.format = format
+        self.data = torch.empty(layout[4], dtype=torch.uint8, device=device)
 
     @property
     def device(self):
@@ -512,6 +523,8 @@ def _status_word(device) -> int:
     """tc_status' address."""
     p = _status_words.get(device.index)
     if p is None:
+        if torch.cuda.is_current_stream_capturing():      # the word would lie in the graph's memory
+            raise ExtensionError("fp4_gemm: the first product on a device cannot be captured; run one before")
         p = _status_words[device.index] = tc_status(device).data_ptr()
     return p
 
@@ -556,7 +569,7 @@ def fp4_dequantize(q: Fp4Matrix, dtype: torch.dtype = torch.float32, out: Option
 
 def fp4_gemm(x: Fp4Matrix, w: Fp4Matrix, out: Optional[torch.Tensor] = None, out_dtype: torch.dtype = torch.float32) -> torch.Tensor:
     """out[M, N] = x[M, K] @ w[N, K]^T of two matrices in the same format, on tcgen05 with block scales, 32-bit sums, for any sizes; the
-    result float32 or bfloat16.  Fast where w has many rows and x is the smaller of the two."""
+    result float32 or bfloat16.  A wait inside the kernel that runs out of time is told by ``check_tc_status``."""
     if x.format != w.format or x.cols != w.cols:
         raise InvalidArgError(f"fp4_gemm: {x.format} [{x.rows}, {x.cols}] and {w.format} [{w.rows}, {w.cols}] do not meet")
     M, N = x.rows, w.rows
