@@ -44,6 +44,7 @@ def lib() -> ctypes.CDLL:
             "llm_model_open_sequence": (c_int32, [PP, I32P]), "llm_model_close_sequence": (c_int32, [PP, c_int32]),
             "llm_model_sequence_length": (c_int32, [PP, c_int32, I32P]),
             "llm_model_step": (c_int32, [PP, c_int32, I32P, I32P, I32P, I32P, I32P, I32P, c_char_p, F32P, F32P, I32P]),
+            "llm_model_step_allowed": (c_int32, [PP, c_int32, I32P, I32P, I32P, I32P, I32P, I32P, c_char_p, F32P, c_void_p, F32P, I32P]),
             "llm_model_step_tokens": (c_int32, [PP, c_int32, I32P, I32P, I32P, I32P, I32P, c_char_p, F32P, PP]),
             "llm_pending_result": (c_int32, [PP, I32P]), "llm_pending_destroy": (c_int32, [PP]),
             "llm_model_result_block": (c_int32, [PP, c_int64, PP, PP]), "llm_block_destroy": (c_int32, [PP]),

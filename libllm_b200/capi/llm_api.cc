@@ -1,6 +1,7 @@
 // The C interface (include/llm.h) over the host library.  Every function catches what the
 // library throws, keeps the message for the calling thread and returns the status, as the
 // reference does at the same boundary (src/libllm/llm.cc:60-71, 134-152).
+#include <algorithm>
 #include <cstring>
 #include <functional>
 #include <memory>
@@ -106,6 +107,21 @@ SamplingParams sampling_of(const Json &kwargs) {
   s.temperature = (float)r.number_or("temperature", 1.0, false);
   s.top_k = (int)r.integer_or("top_k", 50, -(1 << 30));
   s.top_p = (float)r.number_or("top_p", 0.8, false);
+  s.repetition_penalty = (float)r.number_or("repetition_penalty", 1.0, false);
+  s.presence_penalty = (float)r.number_or("presence_penalty", 0.0, false);
+  s.frequency_penalty = (float)r.number_or("frequency_penalty", 0.0, false);
+  const Json &bias = kwargs.get("logit_bias");
+  if (!bias.is_null()) {
+    if (!bias.is_array()) LLM_THROW(InvalidArg, "logit_bias must be a list of [token id, number]");
+    for (const auto &b : bias.items()) {
+      if (!b.is_array() || b.size() != 2 || !b.at(0).is_int() || !b.at(1).is_number() || b.at(0).as_int() < 0 || b.at(0).as_int() > (1ll << 30))
+        LLM_THROW(InvalidArg, "logit_bias must be a list of [token id, number]");
+      s.logit_bias.push_back({(int)b.at(0).as_int(), (float)b.at(1).as_number()});
+    }
+    std::sort(s.logit_bias.begin(), s.logit_bias.end());
+    for (size_t i = 1; i < s.logit_bias.size(); ++i)
+      if (s.logit_bias[i].first == s.logit_bias[i - 1].first) LLM_THROW(InvalidArg, "logit_bias names token %d twice", s.logit_bias[i].first);
+  }
   s.validate();
   return s;
 }
@@ -118,6 +134,7 @@ Engine::Options engine_options(const Json &kwargs) {
   o.max_slots = (int)r.integer_or("max_slots", 0, 0);
   o.max_step_tokens = (int)r.integer_or("max_step_tokens", 8192);
   o.use_graphs = r.boolean_or("use_graphs", true);
+  o.track_history = r.boolean_or("track_history", false);
   o.device = (int)r.integer_or("cuda_device", 0, 0);
   const std::string device = r.string_or("device", "auto");
   if (device == "cpu") LLM_THROW(InvalidArg, "this library has no CPU path: device must be cuda or auto");
@@ -226,7 +243,8 @@ LLM_API int32_t llm_model_destroy(llm_model_t *m) {
 
 namespace {
 const std::initializer_list<const char *> LOAD_KEYS = {"filename", "device", "dtype", "max_tokens", "max_seq_len", "max_slots",
-                                                       "max_step_tokens", "use_graphs", "cuda_device", "strict", "random", "config"};
+                                                       "max_step_tokens", "use_graphs", "cuda_device", "strict", "random", "config",
+                                                       "head", "track_history"};
 
 int64_t positions_for(const Json &kwargs, const Engine::Options &o) {
   // the rotary table is as long as the longest sequence this engine can hold, not as long as the
@@ -252,11 +270,13 @@ LLM_API int32_t llm_model_load(llm_model_t *m, llm_json_t *kwargs) {
       const Json &rnd = r.object("random");
       ConfigReader rr(rnd, "options: random", ErrorKind::InvalidArg);
       model = model_from_config(rr.object("config"), dtype, positions_for(kw, o));
+      model->set_head_format(r.string_or("head", ""));
       model->load_random((uint64_t)rr.integer_or("seed", 0, 0));
       (*m)->path = "<random>";
     } else {
       const std::string folder = r.string("filename");
       model = model_from_config(read_config_json(folder), dtype, positions_for(kw, o));
+      model->set_head_format(r.string_or("head", ""));
       std::unique_ptr<StateMap> state = StateMap::from_folder(folder);
       (*m)->report = model->load(*state, r.boolean_or("strict", true));
       (*m)->path = folder;
@@ -278,6 +298,7 @@ LLM_API int32_t llm_model_load_tensors(llm_model_t *m, llm_json_t *kwargs, int32
     LLM_CUDA(cudaSetDevice(o.device));
     (*m)->engine.reset();
     std::unique_ptr<Model> model = model_from_config(r.object("config"), dtype, positions_for(kw, o));
+    model->set_head_format(r.string_or("head", ""));
     std::unique_ptr<StateMap> state = StateMap::in_memory();
     for (int i = 0; i < n; ++i) {
       StoredTensor t;
@@ -301,6 +322,8 @@ LLM_API int32_t llm_model_get_info(llm_model_t *m, llm_json_t *info) {
     j.set("path", (*m)->path);
     j.set("config", e.model().config());
     j.set("dtype", dtype_name(e.model().dtype()));
+    j.set("head", e.model().head_format());
+    j.set("track_history", e.options().track_history);
     j.set("vocab_size", e.vocab());
     j.set("max_seq_len", e.max_seq_len());
     j.set("capacity_tokens", (int64_t)e.cache().n_pages() * e.cache().page_size());
@@ -343,7 +366,8 @@ LLM_API int32_t llm_model_complete(llm_model_t *m, llm_json_t *kwargs, llm_compl
     Engine &e = engine_of(m);
     if (!comp || !*comp) LLM_THROW(InvalidArg, "the completion handle is null");
     const Json &kw = json_of(kwargs, "options");
-    check_keys(kw, {"temperature", "top_k", "top_p", "prompt_ids", "max_new_tokens", "seed", "stop_token_ids"}, "llm_model_complete");
+    check_keys(kw, {"temperature", "top_k", "top_p", "repetition_penalty", "presence_penalty", "frequency_penalty", "logit_bias", "prompt_ids",
+                    "max_new_tokens", "seed", "stop_token_ids"}, "llm_model_complete");
     ConfigReader r(kw, "options", ErrorKind::InvalidArg);
     std::set<int> stops;
     if (kw.has("stop_token_ids") && !kw.get("stop_token_ids").is_null())
@@ -372,7 +396,8 @@ LLM_API int32_t llm_model_generate(llm_model_t *m, llm_json_t *kwargs, llm_token
   return guard_api([&] {
     Engine &e = engine_of(m);
     const Json &kw = json_of(kwargs, "options");
-    check_keys(kw, {"prompts", "max_new_tokens", "temperature", "top_k", "top_p", "seed", "stop_token_ids", "max_batch"},
+    check_keys(kw, {"prompts", "max_new_tokens", "temperature", "top_k", "top_p", "repetition_penalty", "presence_penalty", "frequency_penalty",
+                    "logit_bias", "seed", "stop_token_ids", "max_batch"},
                "llm_model_generate");
     ConfigReader r(kw, "options", ErrorKind::InvalidArg);
     const Json &ps = kw.get("prompts");
@@ -415,15 +440,21 @@ LLM_API int32_t llm_model_sequence_length(llm_model_t *m, int32_t slot, int32_t 
 LLM_API int32_t llm_model_step(llm_model_t *m, int32_t n_items, const int32_t *slots, const int32_t *n_tokens, const int32_t *tokens,
                                const int32_t *fed_rows, const int32_t *n_want, const int32_t *want, const char *sampling_json,
                                const float *uniforms, float *logits, int32_t *sampled) {
+  return llm_model_step_allowed(m, n_items, slots, n_tokens, tokens, fed_rows, n_want, want, sampling_json, uniforms, nullptr, logits, sampled);
+}
+LLM_API int32_t llm_model_step_allowed(llm_model_t *m, int32_t n_items, const int32_t *slots, const int32_t *n_tokens, const int32_t *tokens,
+                                       const int32_t *fed_rows, const int32_t *n_want, const int32_t *want, const char *sampling_json,
+                                       const float *uniforms, const uint32_t *allowed, float *logits, int32_t *sampled) {
   return guard_api([&] {
     Engine &e = engine_of(m);
     std::vector<StepItem> items;
     build_items(n_items, slots, n_tokens, tokens, fed_rows, n_want, want, &items);
     if (sampling_json) {
       const SamplingParams s = sampling_of(Json::parse(sampling_json, "sampling"));
-      const StepResult r = e.step(items, &s, uniforms);
+      const StepResult r = e.step(items, &s, uniforms, allowed);
       e.read(r, logits, sampled);
     } else {
+      if (allowed) LLM_THROW(InvalidArg, "step: a mask of allowed tokens goes with sampling");
       const StepResult r = e.step(items);
       e.read(r, logits, nullptr);
     }

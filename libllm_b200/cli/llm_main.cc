@@ -3,6 +3,7 @@
 //     llm chat -m FOLDER [-device auto|cuda] [-dtype bfloat16|float32]
 //     llm generate -m FOLDER --prompt-ids 1,2,3 [--prompt-ids ...] [--max-new-tokens N]
 //                  [--temperature T] [--top-k K] [--top-p P] [--seed S] [--no-stop] [--stop-ids a,b]
+//     both:        [--repetition-penalty R] [--presence-penalty P] [--frequency-penalty F] [--head nvfp4|mxfp4]
 //
 // `chat` is the reference's loop (go/bin/chat.go:67-131): a prompt per line, `:new` starts a new
 // session, `:sys TEXT` sets what every session starts with, and after each reply a line with the
@@ -129,7 +130,8 @@ Args parse_args(int argc, char **argv, int first, const std::vector<std::string>
   return a;
 }
 
-const std::vector<std::string> COMMON = {"model", "device", "dtype", "max-tokens", "max-seq-len"};
+const std::vector<std::string> COMMON = {"model", "device", "dtype", "max-tokens", "max-seq-len", "head", "repetition-penalty", "presence-penalty",
+                                         "frequency-penalty"};
 const std::map<std::string, std::string> ALIAS = {{"m", "model"}};
 
 void usage() {
@@ -146,7 +148,25 @@ void common_help() {
           "  -device auto|cuda        inference device (there is no cpu path)\n"
           "  -dtype bfloat16|float32  the engine's type (default bfloat16)\n"
           "  --max-tokens N           tokens the cache holds (default 65536)\n"
-          "  --max-seq-len N          longest sequence (default: the model's)\n");
+          "  --max-seq-len N          longest sequence (default: the model's)\n"
+          "  --head nvfp4|mxfp4       the output matrix in four bits\n"
+          "  --repetition-penalty R   (1) for tokens that the sequence holds\n"
+          "  --presence-penalty P --frequency-penalty F   (0) for tokens that were drawn\n");
+}
+
+const char *const PENALTIES[][2] = {{"repetition-penalty", "repetition_penalty"},
+                                    {"presence-penalty", "presence_penalty"},
+                                    {"frequency-penalty", "frequency_penalty"}};
+bool penalizes(const Args &a) {
+  for (const auto &p : PENALTIES)
+    if (a.has(p[0])) return true;
+  return false;
+}
+std::string penalties_json(const Args &a) {
+  std::string out;
+  for (const auto &p : PENALTIES)
+    if (a.has(p[0])) out += std::string(", \"") + p[1] + "\": " + a.get(p[0], "");
+  return out;
 }
 
 struct Model {
@@ -165,6 +185,8 @@ void load_model(const Args &a, Model *model) {
   kw += "\", \"device\": \"" + device + "\", \"dtype\": \"" + a.get("dtype", "bfloat16") + "\", \"max_tokens\": " +
         a.get("max-tokens", "65536");
   if (a.has("max-seq-len")) kw += ", \"max_seq_len\": " + a.get("max-seq-len", "0");
+  if (a.has("head")) kw += ", \"head\": \"" + a.get("head", "") + "\"";
+  if (penalizes(a)) kw += ", \"track_history\": true";
   kw += "}";
   JsonHandle kwargs(kw);
   check(llm_model_init(&model->m));
@@ -234,7 +256,7 @@ int chat_main(int argc, char **argv) {
     const double t0 = now();
     JsonHandle kwargs("{\"prompt_ids\": " + ids_json(history) + ", \"temperature\": " + a.get("temperature", "1.0") +
                       ", \"top_k\": " + a.get("top-k", "50") + ", \"top_p\": " + a.get("top-p", "0.8") + ", \"max_new_tokens\": " +
-                      a.get("max-new-tokens", "256") + ", \"seed\": " + std::to_string(seed + turn) + "}");
+                      a.get("max-new-tokens", "256") + ", \"seed\": " + std::to_string(seed + turn) + penalties_json(a) + "}");
     llm_completion_t comp = nullptr;
     check(llm_completion_init(&comp));
     std::vector<long long> answer;
@@ -292,7 +314,7 @@ int generate_main(int argc, char **argv) {
   load_model(a, &model);
   std::string kw = "{\"prompts\": " + prompts + ", \"max_new_tokens\": " + a.get("max-new-tokens", "64") + ", \"temperature\": " +
                    a.get("temperature", "1.0") + ", \"top_k\": " + a.get("top-k", "50") + ", \"top_p\": " + a.get("top-p", "0.8") +
-                   ", \"seed\": " + a.get("seed", "0") + ", \"max_batch\": " + a.get("max-batch", "64");
+                   ", \"seed\": " + a.get("seed", "0") + ", \"max_batch\": " + a.get("max-batch", "64") + penalties_json(a);
   if (a.has("no-stop")) kw += ", \"stop_token_ids\": []";
   else if (a.has("stop-ids")) kw += ", \"stop_token_ids\": " + ids_json(parse_ids(a.get("stop-ids", "")));
   kw += "}";

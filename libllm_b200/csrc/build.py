@@ -381,7 +381,7 @@ def main(argv=None) -> int:
     if args.for_model:
         from .. import _lib
         fams = _lib.kernel_families_for(args.for_model, args.dtype)
-        ensure_built(fams)
+        ensure_built(fams + [f for f in args.families if f not in fams])
     elif not args.print_cli or args.families:
         ensure_built(args.families or None)
     build_host()

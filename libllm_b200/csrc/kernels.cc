@@ -939,5 +939,51 @@ void sample(const float *logits, long long stride, int n_rows, int vocab, float 
   LLM_CALL("sampling", llm_sample, logits, stride, n_rows, vocab, temperature, top_k, top_p, uniforms, out, s);
 }
 
+// ---------------------------------------------------------------- logits
+LLM_KERNEL("logits", llm_adjust_logits, const AdjustLogitsCall *)
+LLM_KERNEL("logits", llm_history_place, const int *, const int *, const int *, const int *, const int *, const int *, int, int *, int, int, cudaStream_t)
+LLM_KERNEL("logits", llm_history_drawn, const int *, const int *, const int *, int, int *, int, int, cudaStream_t)
+
+void adjust_logits(const AdjustLogitsCall &call) { LLM_CALL("logits", llm_adjust_logits, &call); }
+void history_place(const int *tokens, const int *fed_tokens, const int *fed_rows, const int *tok_seq, const int *tok_pos, const int *seq_slot, int T,
+                   int *history, int places, int longest, cudaStream_t s) {
+  LLM_CALL("logits", llm_history_place, tokens, fed_tokens, fed_rows, tok_seq, tok_pos, seq_slot, T, history, places, longest, s);
+}
+void history_drawn(const int *drawn, const int *row_slot, const int *drawn_pos, int n, int *history, int places, int longest, cudaStream_t s) {
+  LLM_CALL("logits", llm_history_drawn, drawn, row_slot, drawn_pos, n, history, places, longest, s);
+}
+
+// ---------------------------------------------------------------- four bits
+LLM_KERNEL("fp4", llm_fp4_quantize, const Fp4QuantizeCall *)
+LLM_KERNEL("fp4", llm_fp4_gemm, const Fp4GemmCall *)
+
+namespace {
+struct Fp4Parts {
+  unsigned char *codes, *scales;
+  float *row_scale;
+};
+size_t scales_at(int64_t rows, int64_t cols) { return ((size_t)(rows * ((cols + 31) / 32 * 16)) + 511) / 512 * 512; }
+size_t rows_at(int64_t rows, int64_t cols, Fp4Format f) {
+  return scales_at(rows, cols) + (size_t)((rows + 127) / 128) * (size_t)((cols + 255) / 256) * (f == Fp4Format::NVFP4 ? 2048 : 1024);
+}
+Fp4Parts parts_of(const void *p, int64_t rows, int64_t cols, Fp4Format f) {
+  unsigned char *b = (unsigned char *)p;
+  return {b, b + scales_at(rows, cols), (float *)(b + rows_at(rows, cols, f))};
+}
+}  // namespace
+
+size_t fp4_bytes(int64_t rows, int64_t cols, Fp4Format f) { return rows_at(rows, cols, f) + (size_t)rows * sizeof(float); }
+void fp4_quantize(const Act &x, Fp4Format f, void *dst, cudaStream_t s) {
+  const Fp4Parts q = parts_of(dst, x.rows, x.cols, f);
+  const Fp4QuantizeCall c{code(x.dtype), x.data, x.ld, q.codes, q.scales, q.row_scale, x.rows, x.cols, (long long)f, s};
+  LLM_CALL("fp4", llm_fp4_quantize, &c);
+}
+void fp4_gemm(const void *x, const void *w, int64_t K, Fp4Format f, bool weights_first, const Act &out, int *status, cudaStream_t s) {
+  const Fp4Parts a = parts_of(x, out.rows, K, f), b = parts_of(w, out.cols, K, f);
+  const Fp4GemmCall c{a.codes, a.scales, a.row_scale, b.codes, b.scales, b.row_scale, code(out.dtype), out.data, out.ld, out.rows, out.cols, K, (long long)f,
+                      weights_first ? 1 : 0, status, s};
+  LLM_CALL("fp4", llm_fp4_gemm, &c);
+}
+
 }  // namespace kernels
 }  // namespace llm

@@ -11,6 +11,8 @@
 #include <string>
 #include <vector>
 
+#include "csrc/fp4.h"
+#include "csrc/logits.h"
 #include "util/device.h"
 
 namespace llm {
@@ -370,6 +372,20 @@ void selective_step(const Act &x, const Act &low, int rank, const Weight &w_dt, 
 void argmax(const float *logits, long long stride, int n_rows, int vocab, int *out, cudaStream_t s);
 void sample(const float *logits, long long stride, int n_rows, int vocab, float temperature, int top_k, float top_p,
             const float *uniforms, int *out, cudaStream_t s);
+
+// ---- what a request asks of its logits (csrc/logits.cu)
+void adjust_logits(const AdjustLogitsCall &call);
+// A step's tokens into the histories [places, longest] of their sequences; drawn tokens where they will stand (drawn_pos -1: nowhere).
+void history_place(const int *tokens, const int *fed_tokens, const int *fed_rows, const int *tok_seq, const int *tok_pos, const int *seq_slot, int T,
+                   int *history, int places, int longest, cudaStream_t s);
+void history_drawn(const int *drawn, const int *row_slot, const int *drawn_pos, int n, int *history, int places, int longest, cudaStream_t s);
+
+// ---- matrices in four bits (csrc/fp4.cu): codes, from the next multiple of 512 bytes on the block scales, then the rows' scales
+enum class Fp4Format : int { NVFP4 = 0, MXFP4 = 1 };
+size_t fp4_bytes(int64_t rows, int64_t cols, Fp4Format format);
+void fp4_quantize(const Act &x, Fp4Format format, void *dst, cudaStream_t s);
+// out [M, N] 32-bit or bfloat16 = x [M, K] w [N, K]^T; weights_first: w was complete before the kernel in front of this one could start
+void fp4_gemm(const void *x, const void *w, int64_t K, Fp4Format format, bool weights_first, const Act &out, int *status, cudaStream_t s);
 
 // Kernel launches issued through this file since the process started (graph replays not counted).
 long long launches();

@@ -172,7 +172,49 @@ __global__ void __launch_bounds__(AT) adjust_kernel(Adjust a) {
   }
 }
 
+// A step's tokens into their sequences' histories [places, longest], at their positions: a token that the last step drew (fed_rows[t] >= 0: row
+// of fed_tokens) as its id; one that is brought as ~id, unless the sequence has this very token there already: then it was drawn before.
+__global__ void __launch_bounds__(256) history_place_kernel(const int *tokens, const int *fed_tokens, const int *fed_rows, const int *tok_seq,
+                                                            const int *tok_pos, const int *seq_slot, int T, int *history, int places, int longest) {
+  grid_dependents_launch();
+  grid_dependency_wait();
+  const int t = blockIdx.x * 256 + threadIdx.x;
+  if (t >= T) return;
+  const int place = seq_slot[tok_seq[t]], pos = tok_pos[t], fed = fed_rows ? fed_rows[t] : -1;
+  if (place < 0 || place >= places || pos < 0 || pos >= longest) return;
+  int *at = history + (long long)place * longest + pos;
+  if (fed >= 0) *at = fed_tokens[fed];
+  else if (*at != tokens[t]) *at = ~tokens[t];
+}
+// Drawn tokens where they will stand: row r's at drawn_pos[r] of place row_slot[r]; a position of -1: nowhere.
+__global__ void __launch_bounds__(256) history_drawn_kernel(const int *drawn, const int *row_slot, const int *drawn_pos, int n, int *history, int places,
+                                                            int longest) {
+  grid_dependents_launch();
+  grid_dependency_wait();
+  const int r = blockIdx.x * 256 + threadIdx.x;
+  if (r >= n) return;
+  const int place = row_slot[r], pos = drawn_pos[r];
+  if (place >= 0 && place < places && pos >= 0 && pos < longest) history[(long long)place * longest + pos] = drawn[r];
+}
+
 }  // namespace
+
+LLM_EXPORT int llm_history_place(const int *tokens, const int *fed_tokens, const int *fed_rows, const int *tok_seq, const int *tok_pos,
+                                 const int *seq_slot, int T, int *history, int places, int longest, cudaStream_t stream) {
+  if (T <= 0) return LLM_OK;
+  LLM_REQUIRE(!fed_rows || fed_tokens, "history_place: rows of fed tokens without the tokens");
+  LLM_CHECK_CUDA(llm_launch(history_place_kernel, dim3((T + 255) / 256), dim3(256), 0, stream, tokens, fed_tokens, fed_rows, tok_seq, tok_pos, seq_slot, T,
+                            history, places, longest), "history_place launch");
+  return LLM_OK;
+}
+
+LLM_EXPORT int llm_history_drawn(const int *drawn, const int *row_slot, const int *drawn_pos, int n, int *history, int places, int longest,
+                                 cudaStream_t stream) {
+  if (n <= 0) return LLM_OK;
+  LLM_CHECK_CUDA(llm_launch(history_drawn_kernel, dim3((n + 255) / 256), dim3(256), 0, stream, drawn, row_slot, drawn_pos, n, history, places, longest),
+                 "history_drawn launch");
+  return LLM_OK;
+}
 
 LLM_EXPORT int llm_adjust_logits(const AdjustLogitsCall *call) {
   const AdjustLogitsCall &c = *call;

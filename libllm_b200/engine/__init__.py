@@ -5,6 +5,7 @@ from __future__ import annotations
 
 import ctypes
 import json
+import math
 from array import array
 from ctypes import c_float, c_int32, c_void_p
 from dataclasses import dataclass
@@ -29,16 +30,47 @@ class StepItem:
 @dataclass(frozen=True)
 class SamplingParams:
     """temperature 0 is greedy; top_k 0 draws from the whole vocabulary.  The defaults
-    are the reference's (src/libllm/llm.cc:125-132)."""
+    are the reference's (src/libllm/llm.cc:125-132).
+
+    Before the draw (include/llm.h says it exactly): ``repetition_penalty`` for tokens that the sequence holds, ``presence_penalty`` and
+    ``frequency_penalty`` for those that were drawn (all three need an engine with ``track_history``), and ``logit_bias``, numbers
+    that are added to tokens' logits (a mapping or pairs)."""
     temperature: float = 1.0
     top_k: int = 50
     top_p: float = 0.8
+    repetition_penalty: float = 1.0
+    presence_penalty: float = 0.0
+    frequency_penalty: float = 0.0
+    logit_bias: Any = ()
+
+    def __post_init__(self):
+        bias = self.logit_bias
+        if bias is None:
+            bias = ()
+        elif hasattr(bias, "items"):
+            bias = bias.items()
+        object.__setattr__(self, "logit_bias", tuple((int(t), float(v)) for t, v in bias))
 
     def validate(self) -> None:
         _lib.check(_lib.lib().llm_validate_sampling(float(self.temperature), int(self.top_k), float(self.top_p)))
 
+    def options(self) -> Dict[str, Any]:
+        """As the C interface takes them; what is left at its default is left out."""
+        kw: Dict[str, Any] = dict(temperature=self.temperature, top_k=self.top_k, top_p=self.top_p)
+        for name, default in (("repetition_penalty", 1.0), ("presence_penalty", 0.0), ("frequency_penalty", 0.0)):
+            if getattr(self, name) != default:
+                kw[name] = float(getattr(self, name))
+        if self.logit_bias:
+            kw["logit_bias"] = self.logit_bias
+        for name in ("repetition_penalty", "presence_penalty", "frequency_penalty"):
+            if not math.isfinite(kw.get(name, 0.0)):
+                raise InvalidArgError(f"{name} must be a finite number")
+        if not all(math.isfinite(v) for _, v in self.logit_bias):
+            raise InvalidArgError("logit_bias holds a number that is not finite")
+        return kw
+
     def to_json(self) -> bytes:
-        return json.dumps(dict(temperature=self.temperature, top_k=self.top_k, top_p=self.top_p)).encode()
+        return json.dumps(self.options()).encode()
 
 
 GREEDY = SamplingParams(temperature=0.0, top_k=1, top_p=1.0)
@@ -126,7 +158,8 @@ class Engine:
 
     # ---------------------------------------------------------------- making one
     @staticmethod
-    def _options(dtype, max_tokens, max_seq_len, max_slots, max_step_tokens, use_graphs, cuda_device, strict) -> Dict[str, Any]:
+    def _options(dtype, max_tokens, max_seq_len, max_slots, max_step_tokens, use_graphs, cuda_device, strict, head,
+                 track_history) -> Dict[str, Any]:
         kw: Dict[str, Any] = dict(dtype=str(dtype).replace("torch.", ""), max_tokens=int(max_tokens),
                                   max_step_tokens=int(max_step_tokens), use_graphs=bool(use_graphs),
                                   cuda_device=int(cuda_device), strict=bool(strict))
@@ -134,12 +167,16 @@ class Engine:
             kw["max_seq_len"] = int(max_seq_len)
         if max_slots:
             kw["max_slots"] = int(max_slots)
+        if head:
+            kw["head"] = str(head)
+        if track_history:
+            kw["track_history"] = True
         return kw
 
     @classmethod
     def _load(cls, kw: Dict[str, Any], config_json: dict, loader: Callable[[c_void_p, _lib.Json], int], keep=None) -> "Engine":
         L = _lib.lib()
-        _lib.use_families(_lib.describe_model(config_json, kw["dtype"])["kernel_families"])
+        _lib.use_families(_lib.describe_model(config_json, kw["dtype"])["kernel_families"] + (["fp4"] if "head" in kw else []))
         h = c_void_p()
         _lib.check(L.llm_model_init(ctypes.byref(h)))
         try:
@@ -152,9 +189,12 @@ class Engine:
     @classmethod
     def from_folder(cls, folder: str, dtype="bfloat16", max_tokens: int = 65536, max_seq_len: Optional[int] = None,
                     max_slots: Optional[int] = None, max_step_tokens: int = 8192, use_graphs: bool = True,
-                    cuda_device: int = 0, strict: bool = True, device: str = "auto") -> "Engine":
+                    cuda_device: int = 0, strict: bool = True, device: str = "auto", head: Optional[str] = None,
+                    track_history: bool = False) -> "Engine":
+        """``head``: "nvfp4" or "mxfp4" brings the output matrix and the rows it meets into four bits; ``track_history``: the device keeps
+        every sequence's tokens, which the penalties of SamplingParams need (4 bytes x slots x max_seq_len)."""
         import os
-        kw = cls._options(dtype, max_tokens, max_seq_len, max_slots, max_step_tokens, use_graphs, cuda_device, strict)
+        kw = cls._options(dtype, max_tokens, max_seq_len, max_slots, max_step_tokens, use_graphs, cuda_device, strict, head, track_history)
         kw["filename"] = folder
         kw["device"] = device
         path = os.path.join(folder, "config.json")
@@ -172,20 +212,21 @@ class Engine:
     @classmethod
     def from_random(cls, config_json: dict, seed: int = 0, dtype="bfloat16", max_tokens: int = 65536,
                     max_seq_len: Optional[int] = None, max_slots: Optional[int] = None, max_step_tokens: int = 8192,
-                    use_graphs: bool = True, cuda_device: int = 0) -> "Engine":
+                    use_graphs: bool = True, cuda_device: int = 0, head: Optional[str] = None, track_history: bool = False) -> "Engine":
         """The random-weights mode without a folder: tensors are drawn on the device (matrices
         N(0, 0.02), norm weights 1 + U(-0.1, 0.1)) from ``seed``."""
-        kw = cls._options(dtype, max_tokens, max_seq_len, max_slots, max_step_tokens, use_graphs, cuda_device, True)
+        kw = cls._options(dtype, max_tokens, max_seq_len, max_slots, max_step_tokens, use_graphs, cuda_device, True, head, track_history)
         kw["random"] = dict(config=config_json, seed=int(seed))
         return cls._load(kw, config_json, lambda h, j: _lib.lib().llm_model_load(ctypes.byref(h), j.ref))
 
     @classmethod
     def from_tensors(cls, config_json: dict, tensors: Dict[str, Any], dtype="bfloat16", max_tokens: int = 65536,
                      max_seq_len: Optional[int] = None, max_slots: Optional[int] = None, max_step_tokens: int = 8192,
-                     use_graphs: bool = True, cuda_device: int = 0, strict: bool = True) -> "Engine":
+                     use_graphs: bool = True, cuda_device: int = 0, strict: bool = True, head: Optional[str] = None,
+                     track_history: bool = False) -> "Engine":
         """``tensors``: name -> numpy array (float32, float16, int32, ...) or torch tensor on the
         CPU (bfloat16 too).  They are read while this call runs and not kept."""
-        kw = cls._options(dtype, max_tokens, max_seq_len, max_slots, max_step_tokens, use_graphs, cuda_device, strict)
+        kw = cls._options(dtype, max_tokens, max_seq_len, max_slots, max_step_tokens, use_graphs, cuda_device, strict, head, track_history)
         kw["config"] = config_json
         n, c_names, c_dtypes, c_shapes, c_ndims, c_ptrs, keep = _lib.host_tensors(tensors)
 
@@ -269,11 +310,13 @@ class Engine:
         return np.asarray(_Block(block, data.value, shape)) if block else np.empty(shape, dtype=np.float32)
 
     def step(self, items: Sequence[StepItem], sampling: Optional[SamplingParams] = None,
-             uniforms: Optional[Sequence[float]] = None, return_logits: bool = True):
+             uniforms: Optional[Sequence[float]] = None, return_logits: bool = True, allowed: Optional[np.ndarray] = None):
         """Runs the items' tokens and returns the logits at the wanted places, float32
         [wanted, vocab] in the order of the items and of their ``want``.  With ``sampling`` it
         returns (logits or None, tokens): a token drawn at each wanted place; ``uniforms`` then
-        holds one number in [0, 1) per wanted place.
+        holds one number in [0, 1) per wanted place.  ``allowed`` (with ``sampling``): which tokens may be drawn, bool
+        [wanted, vocab], or the same as bits, uint32 or int32 [wanted, (vocab + 31) // 32] with token v in bit v % 32 of word
+        v // 32.  The logits are the model's own, without penalties, bias or mask.
 
         The logits may lie in page-locked memory that the engine lends for as long as an array looks at any of them, and such an
         array cannot be resized in place: copy the rows that are to be kept for long."""
@@ -282,20 +325,34 @@ class Engine:
         W = len(want)
         if sampling is not None and uniforms is not None and len(uniforms) != W:
             raise InvalidArgError("one uniform number per wanted place is needed")
+        mask = None if allowed is None else self._mask_words(allowed, W)
+        if mask is not None and sampling is None:
+            raise InvalidArgError("a mask of allowed tokens goes with sampling")
         logits = self._rows(W) if (return_logits or sampling is None) else None
         sampled = np.empty(max(W, 1), dtype=np.int32) if sampling is not None else None
         uni = None
         if sampling is not None and uniforms is not None:
             uni = (c_float * max(1, W))(*[float(u) for u in uniforms])
-        _lib.check(_lib.lib().llm_model_step(
+        _lib.check(_lib.lib().llm_model_step_allowed(
             ctypes.byref(self._h), len(items), _lib.int32_array(slots), _lib.int32_array(n_tok), _pointer(toks),
             _lib.int32_array(fed), _lib.int32_array(n_want), _lib.int32_array(want),
-            sampling.to_json() if sampling is not None else None, uni,
+            sampling.to_json() if sampling is not None else None, uni, mask.ctypes.data if mask is not None and mask.size else None,
             logits.ctypes.data_as(ctypes.POINTER(c_float)) if logits is not None else None,
             sampled.ctypes.data_as(ctypes.POINTER(c_int32)) if sampled is not None else None))
         if sampling is None:
             return logits
         return logits, sampled[:W]
+
+    def _mask_words(self, allowed, rows: int) -> np.ndarray:
+        mask = np.asarray(allowed)
+        words = (self.vocab + 31) // 32
+        if mask.dtype == np.bool_ and mask.shape == (rows, self.vocab):
+            padded = np.zeros((rows, words * 32), dtype=np.bool_)
+            padded[:, :self.vocab] = mask
+            return np.packbits(padded, axis=1, bitorder="little").view("<u4")
+        if mask.dtype in (np.uint32, np.int32) and mask.shape == (rows, words):
+            return np.ascontiguousarray(mask)
+        raise InvalidArgError(f"allowed is bool [{rows}, {self.vocab}] or uint32 [{rows}, {words}], got {mask.dtype} {list(mask.shape)}")
 
     def step_tokens(self, items: Sequence[StepItem], sampling: SamplingParams,
                     uniforms: Optional[Sequence[float]] = None) -> PendingTokens:
@@ -324,8 +381,7 @@ class Engine:
         ``on_token(request index, token)`` is called as tokens arrive."""
         kw: Dict[str, Any] = dict(prompts=[[int(t) for t in p] for p in prompts],
                                   max_new_tokens=max_new_tokens if isinstance(max_new_tokens, int) else list(max_new_tokens),
-                                  temperature=sampling.temperature, top_k=sampling.top_k, top_p=sampling.top_p,
-                                  seed=int(seed), max_batch=int(max_batch))
+                                  seed=int(seed), max_batch=int(max_batch), **sampling.options())
         if stop_tokens is not None:
             kw["stop_token_ids"] = [int(t) for t in stop_tokens]
         cb, raised = None, []
@@ -347,8 +403,8 @@ class Engine:
                  max_new_tokens: int = 1 << 30, seed: int = 0, stop_tokens: Optional[Iterable[int]] = None) -> Iterator[int]:
         """One prompt, token by token (the reference's completion handle, src/libllm/llm.cc:266-308)."""
         L = _lib.lib()
-        kw: Dict[str, Any] = dict(prompt_ids=[int(t) for t in prompt], temperature=sampling.temperature, top_k=sampling.top_k,
-                                  top_p=sampling.top_p, max_new_tokens=int(min(max_new_tokens, 1 << 30)), seed=int(seed))
+        kw: Dict[str, Any] = dict(prompt_ids=[int(t) for t in prompt], max_new_tokens=int(min(max_new_tokens, 1 << 30)), seed=int(seed),
+                                  **sampling.options())
         if stop_tokens is not None:
             kw["stop_token_ids"] = [int(t) for t in stop_tokens]
         comp = c_void_p()

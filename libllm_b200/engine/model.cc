@@ -115,8 +115,20 @@ std::vector<TensorNeed> Model::tensor_needs() const {
   return needs;
 }
 
+namespace {
+kernels::Fp4Format fp4_format(const std::string &name) { return name == "mxfp4" ? kernels::Fp4Format::MXFP4 : kernels::Fp4Format::NVFP4; }
+}  // namespace
+
+void Model::set_head_format(const std::string &format) {
+  if (!format.empty() && format != "nvfp4" && format != "mxfp4")
+    LLM_THROW(InvalidArg, "the output matrix has no format '%s' (nvfp4 or mxfp4)", format.c_str());
+  if (loaded_) LLM_THROW(InvalidArg, "the output matrix's format is chosen before the weights are loaded");
+  head_format_ = format;
+}
+
 std::vector<std::string> Model::kernel_families() const {
-  std::set<std::string> fams = {"elementwise", "sampling"};
+  std::set<std::string> fams = {"elementwise", "sampling", "logits"};
+  if (!head_format_.empty()) fams.insert("fp4");
   for (auto &f : product_families(dtype_)) fams.insert(f);
   for (const auto &l : layers_)
     for (auto &f : l->kernel_families()) fams.insert(f);
@@ -145,6 +157,19 @@ void Model::load_with(const Loader &loader) {
   } else {
     head_own_ = loader.fetch(needs.back());
     head_ = &head_own_;
+  }
+  if (!head_format_.empty()) {
+    LLM_CUDA(cudaDeviceSynchronize());
+    Act w;
+    w.data = head_->data();
+    w.dtype = head_->dtype;
+    w.rows = head_->rows;
+    w.cols = w.ld = head_->cols;
+    const kernels::Fp4Format f = fp4_format(head_format_);
+    head_four_.allocate(kernels::fp4_bytes(w.rows, w.cols, f));
+    kernels::fp4_quantize(w, f, head_four_.get(), nullptr);
+    LLM_CUDA(cudaDeviceSynchronize());
+    head_own_.buf.release();                       // a tied matrix stays: it is the token table
   }
   LLM_CUDA(cudaDeviceSynchronize());
   loaded_ = true;
@@ -294,8 +319,18 @@ Act Model::forward(StepContext &ctx, KVCache &cache, const std::vector<const int
     stream.picked = true;
   }
   Act h = stream.picked ? final_norm_->forward(ctx, stream) : final_norm_->forward(ctx, stream, ctx.want_rows, ctx.n_want);
-  Act logits = linear(ctx, h, *head_, nullptr, DType::F32);
-  flush_chain(ctx);
+  Act logits;
+  if (head_format_.empty()) {
+    logits = linear(ctx, h, *head_, nullptr, DType::F32);
+    flush_chain(ctx);
+  } else {
+    flush_chain(ctx);
+    const kernels::Fp4Format f = fp4_format(head_format_);
+    void *rows = ctx.arena->alloc(kernels::fp4_bytes(h.rows, h.cols, f), 512);
+    logits = ctx.arena->act(DType::F32, h.rows, spec_.vocab_size);
+    kernels::fp4_quantize(h, f, rows, ctx.stream);
+    kernels::fp4_gemm(rows, head_four_.get(), h.cols, f, true, logits, ctx.tc_status, ctx.stream);
+  }
   if (spec_.logit_scale != 1.0 || spec_.logit_softcap > 0.0)
     kernels::logit_transform((float *)logits.data, logits.rows * logits.cols, (float)spec_.logit_scale, (float)spec_.logit_softcap,
                              ctx.stream);

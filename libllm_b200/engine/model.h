@@ -38,6 +38,10 @@ class Model {
   // Whether steps of single tokens may be captured as CUDA graphs (every part says so).
   bool capturable() const;
 
+  // Before load: the output matrix is brought into four bits ("nvfp4", "mxfp4"; "": it stays as it is) and the last rows with it.
+  void set_head_format(const std::string &format);
+  const std::string &head_format() const { return head_format_; }
+
   // Checks the tensors against the needs (one error for everything that does not fit) and brings
   // them to the device.  Returns the report (ignored and, when not strict, unexpected tensors).
   WeightsReport load(const StateMap &state, bool strict = true);
@@ -78,6 +82,8 @@ class Model {
   TensorNeed pairs_need() const;
   TensorNeed token_table_need() const;
   const Weight *head_ = nullptr;
+  std::string head_format_;                        // set_head_format()
+  DeviceBuffer head_four_;                         // the output matrix in four bits (csrc/fp4.cu)
   bool loaded_ = false;
 };
 

@@ -1,6 +1,7 @@
 #include "engine/step.h"
 
 #include <algorithm>
+#include <cmath>
 #include <cstring>
 #include <numeric>
 #include <set>
@@ -16,6 +17,11 @@ void SamplingParams::validate() const {
   if (top_k < 0 || top_k > 1024) LLM_THROW(InvalidArg, "top_k must lie in 0..1024 (0: the whole vocabulary)");
   if (!(top_p > 0)) LLM_THROW(InvalidArg, "top_p must be positive");
   if (top_k == 0 && top_p < 1.0f && temperature > 0) LLM_THROW(InvalidArg, "top_p below 1 needs a top_k");
+  if (!(repetition_penalty > 0) || !std::isfinite(repetition_penalty)) LLM_THROW(InvalidArg, "repetition_penalty must be a positive number");
+  if (!std::isfinite(presence_penalty) || !std::isfinite(frequency_penalty))
+    LLM_THROW(InvalidArg, "presence_penalty and frequency_penalty must be numbers");
+  for (const auto &b : logit_bias)
+    if (!std::isfinite(b.second)) LLM_THROW(InvalidArg, "logit_bias: token %d has no finite number", b.first);
 }
 
 bool Engine::GraphKey::operator<(const GraphKey &o) const {
@@ -23,6 +29,7 @@ bool Engine::GraphKey::operator<(const GraphKey &o) const {
   if (width != o.width) return width < o.width;
   if (sampled != o.sampled) return sampled < o.sampled;
   if (!sampled) return false;
+  if (masked != o.masked) return masked < o.masked;
   return sampling < o.sampling;
 }
 
@@ -32,18 +39,21 @@ bool Engine::GraphKey::operator<(const GraphKey &o) const {
 // uniform numbers, the rows of fed tokens, and a page table per cache group.
 class Engine::Descriptor {
  public:
-  enum Field { Tokens, TokSeq, TokPos, SeqStart, SeqPast, SeqSlot, Want, Uniforms, Fed, Tables };
+  // RowSlot, RowLen, DrawnPos (engines that track histories): a wanted row's slot, the tokens its sequence holds up to it, and where in the sequence a
+  // token drawn from it will stand (-1: it is not the last of the tokens that the step was given).
+  enum Field { Tokens, TokSeq, TokPos, SeqStart, SeqPast, SeqSlot, Want, Uniforms, Fed, RowSlot, RowLen, DrawnPos, Tables };
 
   Descriptor() { LLM_CUDA(cudaEventCreateWithFlags(&copied_, cudaEventDisableTiming)); }
   ~Descriptor() { cudaEventDestroy(copied_); }
 
-  void shape(int T, int B, int W, const std::vector<int> &widths) {
+  void shape(int T, int B, int W, const std::vector<int> &widths, bool history) {
     wait_host_free();
     n_tokens = T;
     n_seqs = B;
     n_want = W;
     this->widths = widths;
-    sizes_ = {T, T, T, B + 1, B, B, W, std::max(B, W), T};
+    const int H = history ? W : 0;
+    sizes_ = {T, T, T, B + 1, B, B, W, std::max(B, W), T, H, H, H};
     for (int w : widths) sizes_.push_back(B * w);
     offsets_.assign(1, 0);
     for (int s : sizes_) offsets_.push_back(offsets_.back() + (size_t)((s + 3) / 4 * 4));
@@ -100,6 +110,7 @@ struct Engine::DecodeGraph {
   int batch = 0, width = 0;
   bool sampled = false;
   SamplingParams sampling;
+  DeviceBuffer allowed;              // a masked step's words, brought in ahead of the graph
   Descriptor desc;
   Arena arena{(size_t)16 << 20};
   cudaGraph_t graph = nullptr;
@@ -142,6 +153,10 @@ Engine::Engine(std::unique_ptr<Model> model, const Options &options) : model_(st
     LLM_CUDA(cudaEventCreateWithFlags(&t.done, cudaEventDisableTiming));
   }
   status_host_.allocate(sizeof(int) * ((size_t)last_capacity_ + 1));
+  if (opt_.track_history) {
+    history_places_ = cache_->slots().n_slots();
+    history_.allocate((size_t)history_places_ * (size_t)max_seq_len_ * sizeof(int));
+  }
   // three results of 64 rows of logits (a caller reads one while the next is computed), at most 96 MB
   host_pool_.reset(new HostPool(std::min((size_t)96 << 20, 3 * 64 * sizeof(float) * (size_t)vocab())));
 }
@@ -159,7 +174,16 @@ void Engine::make_current() const { LLM_CUDA(cudaSetDevice(opt_.device)); }
 
 int Engine::open_sequence() {
   make_current();
-  return cache_->open(stream_);
+  const int slot = cache_->open(stream_);
+  if (opt_.track_history) {
+    // no token's id: what another sequence left in the slot is not taken for this one's
+    const cudaError_t e = cudaMemsetAsync(history_.as<int>() + (size_t)slot * (size_t)max_seq_len_, 0x80, (size_t)max_seq_len_ * sizeof(int), stream_);
+    if (e != cudaSuccess) {
+      cache_->close(slot);
+      LLM_CUDA(e);
+    }
+  }
+  return slot;
 }
 void Engine::close_sequence(int slot) { cache_->close(slot); }
 void Engine::synchronize() {
@@ -209,6 +233,19 @@ void Engine::validate(const std::vector<StepItem> &items) const {
   }
 }
 
+void Engine::validate_adjustments(const std::vector<StepItem> &items, const SamplingParams &s) const {
+  for (const auto &b : s.logit_bias)
+    if (b.first < 0 || b.first >= vocab())
+      LLM_THROW(InvalidArg, "logit_bias: token id %d outside the vocabulary (%lld)", b.first, (long long)vocab());
+  if (!s.penalizes()) return;
+  if (!opt_.track_history) LLM_THROW(InvalidArg, "penalties need an engine that was loaded with track_history");
+  for (const auto &it : items)
+    for (int w : it.want)
+      if (w + 1 != (int)it.tokens.size())
+        LLM_THROW(InvalidArg, "slot %d: with penalties a token is drawn behind the last token of a step, not at place %d of %zu", it.slot, w,
+                  it.tokens.size());
+}
+
 // ---------------------------------------------------------------- descriptor
 void Engine::fill(Descriptor &d, const std::vector<Piece> &pieces, const std::vector<StepItem> &items,
                   const std::vector<int> &want_rows, const float *uniforms, int n_uniforms) {
@@ -241,6 +278,22 @@ void Engine::fill(Descriptor &d, const std::vector<Piece> &pieces, const std::ve
   }
   seq_start[pieces.size()] = o;
   std::copy(want_rows.begin(), want_rows.end(), d.host(Descriptor::Want));
+  if (d.size(Descriptor::RowSlot) > 0) {
+    int *drawn_pos = d.host(Descriptor::DrawnPos);
+    std::vector<int> drawn_by(pieces.size(), -1);
+    for (size_t r = 0; r < want_rows.size(); ++r) {
+      const int b = tok_seq[want_rows[r]], len = tok_pos[want_rows[r]] + 1;
+      const Piece &p = pieces[(size_t)b];
+      const StepItem &it = items[(size_t)p.index];
+      d.host(Descriptor::RowSlot)[r] = p.slot;
+      d.host(Descriptor::RowLen)[r] = len;
+      // (a captured step draws for every sequence, but what one that wants nothing "drew" is nobody's)
+      drawn_pos[r] = len == p.past + (int)it.tokens.size() && !it.want.empty() ? len : -1;
+      if (drawn_pos[r] < 0) continue;
+      if (drawn_by[(size_t)b] >= 0) drawn_pos[drawn_by[(size_t)b]] = -1;       // the same place asked for twice: the last draw stands
+      drawn_by[(size_t)b] = (int)r;
+    }
+  }
   if (uniforms) memcpy(d.host(Descriptor::Uniforms), uniforms, sizeof(float) * (size_t)n_uniforms);
   for (size_t g = 0; g < d.widths.size(); ++g) cache_->page_table((int)g, slots, d.widths[g], d.host(Descriptor::Tables + (int)g));
 }
@@ -288,18 +341,72 @@ StepContext Engine::context(Descriptor &d, const std::vector<Piece> &pieces, int
   return ctx;
 }
 
-void Engine::sample(const Act &logits, const SamplingParams &s, const float *uniforms_dev, int *out) {
-  if (s.greedy()) kernels::argmax((const float *)logits.data, logits.ld, (int)logits.rows, (int)logits.cols, out, stream_);
-  else kernels::sample((const float *)logits.data, logits.ld, (int)logits.rows, (int)logits.cols, s.temperature, s.top_k, s.top_p,
-                       uniforms_dev, out, stream_);
+void Engine::place_history(Descriptor &d) {
+  if (opt_.track_history)
+    kernels::history_place(d.dev(Descriptor::Tokens), last_tokens_.as<int>(), d.dev(Descriptor::Fed), d.dev(Descriptor::TokSeq), d.dev(Descriptor::TokPos),
+                           d.dev(Descriptor::SeqSlot), d.n_tokens, history_.as<int>(), history_places_, (int)max_seq_len_, stream_);
+}
+
+// The step's bias where the kernel reads it; kept while steps ask for the same one.
+void Engine::bring_bias(const SamplingParams &s) {
+  if (s.logit_bias.empty() || (bias_ && s.logit_bias == bias_now_)) return;
+  std::vector<float> dense((size_t)vocab(), 0.f);
+  for (const auto &b : s.logit_bias) dense[(size_t)b.first] = b.second;
+  if (!bias_) bias_.allocate(dense.size() * sizeof(float));
+  bias_now_.clear();
+  LLM_CUDA(cudaMemcpyAsync(bias_.get(), dense.data(), dense.size() * sizeof(float), cudaMemcpyHostToDevice, stream_));
+  LLM_CUDA(cudaStreamSynchronize(stream_));          // `dense` has been read
+  bias_now_ = s.logit_bias;
+}
+
+void Engine::sample(const Act &logits, const SamplingParams &s, Descriptor &d, const unsigned *allowed_dev, Arena *arena, int *out) {
+  const float *rows = (const float *)logits.data;
+  int64_t ld = logits.ld;
+  if (s.penalizes() || !s.logit_bias.empty() || allowed_dev) {
+    AdjustLogitsCall c = {};
+    c.logits = rows;
+    c.ld = ld;
+    c.B = logits.rows;
+    c.V = c.ldo = logits.cols;
+    c.out = arena->alloc_n<float>((size_t)(c.B * c.V));
+    if (s.penalizes()) {
+      c.history = history_.as<int>();
+      c.ldh = c.longest = max_seq_len_;
+      c.places = history_places_;
+      c.slots = d.dev(Descriptor::RowSlot);
+      c.lengths = d.dev(Descriptor::RowLen);
+    }
+    c.repetition_all = s.repetition_penalty;
+    c.presence_all = s.presence_penalty;
+    c.frequency_all = s.frequency_penalty;
+    c.bias = s.logit_bias.empty() ? nullptr : bias_.as<float>();
+    c.allowed = allowed_dev;
+    c.ld_allowed = (logits.cols + 31) / 32;
+    c.stream = stream_;
+    kernels::adjust_logits(c);
+    rows = c.out;
+    ld = c.ldo;
+  }
+  const float *uniforms_dev = (const float *)d.dev(Descriptor::Uniforms);
+  if (s.greedy()) kernels::argmax(rows, ld, (int)logits.rows, (int)logits.cols, out, stream_);
+  else kernels::sample(rows, ld, (int)logits.rows, (int)logits.cols, s.temperature, s.top_k, s.top_p, uniforms_dev, out, stream_);
+  if (opt_.track_history)
+    kernels::history_drawn(out, d.dev(Descriptor::RowSlot), d.dev(Descriptor::DrawnPos), (int)logits.rows, history_.as<int>(), history_places_,
+                           (int)max_seq_len_, stream_);
 }
 
 // ---------------------------------------------------------------- the step
-StepResult Engine::step(const std::vector<StepItem> &items, const SamplingParams *sampling, const float *uniforms) {
+StepResult Engine::step(const std::vector<StepItem> &items, const SamplingParams *sampling, const float *uniforms, const uint32_t *allowed) {
   make_current();
   if (items.empty()) LLM_THROW(InvalidArg, "a step needs at least one sequence");
   validate(items);
-  if (sampling) sampling->validate();
+  if (sampling) {
+    sampling->validate();
+    validate_adjustments(items, *sampling);
+    bring_bias(*sampling);
+  } else if (allowed) {
+    LLM_THROW(InvalidArg, "a mask of allowed tokens goes with sampling");
+  }
   // Pages first: either the whole step fits the cache or nothing changes.
   std::vector<std::pair<int, int>> growth;
   bool decode_only = true;
@@ -310,9 +417,9 @@ StepResult Engine::step(const std::vector<StepItem> &items, const SamplingParams
   cache_->reserve(growth);
   StepResult out;
   if (decode_only && opt_.use_graphs && model_->capturable() && (int)items.size() <= opt_.max_step_tokens)
-    out = run_decode_graph(items, sampling, uniforms);
+    out = run_decode_graph(items, sampling, uniforms, allowed);
   else
-    out = run_eager(items, sampling, uniforms);
+    out = run_eager(items, sampling, uniforms, allowed);
   ++steps_run_;
   return out;
 }
@@ -329,7 +436,7 @@ void Engine::read(const StepResult &r, float *logits, int *tokens) {
 }
 
 // ---------------------------------------------------------------- eager path (prompts, mixed steps)
-StepResult Engine::run_eager(const std::vector<StepItem> &items, const SamplingParams *sampling, const float *uniforms) {
+StepResult Engine::run_eager(const std::vector<StepItem> &items, const SamplingParams *sampling, const float *uniforms, const uint32_t *allowed) {
   // Pieces: the step's tokens in launch sequences of at most max_step_tokens, cut inside a prompt
   // where need be.
   std::vector<std::vector<Piece>> chunks(1);
@@ -361,6 +468,7 @@ StepResult Engine::run_eager(const std::vector<StepItem> &items, const SamplingP
   float *all_logits = W ? results_.alloc_n<float>((size_t)W * (size_t)V) : nullptr;
   int *all_tokens = (sampling && W) ? results_.alloc_n<int>((size_t)W) : nullptr;
 
+  bool masked = false;
   for (const auto &pieces : chunks) {
     int T = 0;
     for (const auto &p : pieces) T += p.count;
@@ -386,7 +494,7 @@ StepResult Engine::run_eager(const std::vector<StepItem> &items, const SamplingP
     const int width = std::max(8, (need_pages + 7) / 8 * 8);
     Descriptor &d = *eager_desc_[eager_turn_];
     eager_turn_ = (eager_turn_ + 1) % eager_desc_.size();
-    d.shape(T, (int)pieces.size(), (int)want_rows.size(), std::vector<int>(cache_->groups().size(), width));
+    d.shape(T, (int)pieces.size(), (int)want_rows.size(), std::vector<int>(cache_->groups().size(), width), opt_.track_history);
     fill(d, pieces, items, want_rows, uni.data(), (int)uni.size());
     d.upload(stream_);
     last_h2d_ = (long long)(d.words() * sizeof(int));
@@ -399,10 +507,19 @@ StepResult Engine::run_eager(const std::vector<StepItem> &items, const SamplingP
     ctx.layer_arenas[0] = &layer_scratch_[0];
     ctx.layer_arenas[1] = &layer_scratch_[1];
     Act logits = model_->forward(ctx, *cache_, tables, width, last_tokens_.as<int>(), d.dev(Descriptor::Fed));
+    place_history(d);
     int *chunk_tokens = nullptr;
     if (sampling && !want_rows.empty()) {
       chunk_tokens = scratch_.alloc_n<int>(want_rows.size());
-      sample(logits, *sampling, (const float *)d.dev(Descriptor::Uniforms), chunk_tokens);
+      unsigned *words = nullptr;
+      if (allowed) {
+        const size_t n = (size_t)((V + 31) / 32);
+        words = scratch_.alloc_n<unsigned>(global.size() * n);
+        for (size_t i = 0; i < global.size(); ++i)
+          LLM_CUDA(cudaMemcpyAsync(words + i * n, allowed + (size_t)global[i] * n, n * sizeof(unsigned), cudaMemcpyHostToDevice, stream_));
+        masked = true;
+      }
+      sample(logits, *sampling, d, words, &scratch_, chunk_tokens);
     }
     // into the step's result, in runs of rows that are neighbours there too
     for (size_t a = 0; a < global.size();) {
@@ -416,6 +533,7 @@ StepResult Engine::run_eager(const std::vector<StepItem> &items, const SamplingP
     }
     for (const auto &p : pieces) cache_->commit(p.slot, p.past + p.start + p.count);
   }
+  if (masked) LLM_CUDA(cudaStreamSynchronize(stream_));        // `allowed` has been read
   StepResult r;
   r.logits = all_logits;
   r.n_rows = W;
@@ -435,14 +553,16 @@ Act Engine::graph_body(DecodeGraph &g) {
   StepContext ctx = context(d, pieces, g.batch, true, g.width * opt_.page_size, &g.arena, &tables);
   ctx.captured = true;
   Act logits = model_->forward(ctx, *cache_, tables, g.width, last_tokens_.as<int>(), d.dev(Descriptor::Fed));
+  place_history(d);
   if (g.sampled) {
-    sample(logits, g.sampling, (const float *)d.dev(Descriptor::Uniforms), last_tokens_.as<int>());
+    sample(logits, g.sampling, d, g.allowed.as<unsigned>(), &g.arena, last_tokens_.as<int>());
     kernels::gather_words(last_tokens_.as<int>(), g.batch, status_.as<int>(), 1, g.host_tokens.as<int>(), stream_);
   }
   return logits;
 }
 
-StepResult Engine::run_decode_graph(const std::vector<StepItem> &items, const SamplingParams *sampling, const float *uniforms) {
+StepResult Engine::run_decode_graph(const std::vector<StepItem> &items, const SamplingParams *sampling, const float *uniforms,
+                                    const uint32_t *allowed) {
   const int B = (int)items.size();
   std::vector<Piece> pieces;
   int need_pages = 1;
@@ -453,7 +573,7 @@ StepResult Engine::run_decode_graph(const std::vector<StepItem> &items, const Sa
   }
   int width = 8;
   while (width < need_pages) width *= 2;
-  GraphKey key{B, width, sampling != nullptr, sampling ? *sampling : SamplingParams()};
+  GraphKey key{B, width, sampling != nullptr, allowed != nullptr, sampling ? *sampling : SamplingParams()};
   // Each shape has two graphs taken in turn: while one step runs, the next one's descriptor is
   // written into the other graph's staging, and a step's tokens are read while the other runs.
   int &turn = graph_turn_[key];
@@ -467,7 +587,8 @@ StepResult Engine::run_decode_graph(const std::vector<StepItem> &items, const Sa
     slot->width = width;
     slot->sampled = sampling != nullptr;
     if (sampling) slot->sampling = *sampling;
-    slot->desc.shape(B, B, B, std::vector<int>(cache_->groups().size(), width));
+    slot->desc.shape(B, B, B, std::vector<int>(cache_->groups().size(), width), opt_.track_history);
+    if (allowed) slot->allowed.allocate((size_t)B * (size_t)((vocab() + 31) / 32) * sizeof(unsigned));
     if (sampling) slot->host_tokens.allocate(sizeof(int) * ((size_t)B + 1));
   }
   DecodeGraph &g = *slot;
@@ -484,6 +605,13 @@ StepResult Engine::run_decode_graph(const std::vector<StepItem> &items, const Sa
     }
   g.desc.wait_host_free();
   fill(g.desc, pieces, items, all_rows, uni.data(), B);
+  if (allowed) {
+    // a sequence that wants nothing gets no words of its own: what is drawn for it is not handed out
+    const size_t n = (size_t)((vocab() + 31) / 32);
+    for (size_t i = 0; i < rows.size(); ++i)
+      LLM_CUDA(cudaMemcpyAsync(g.allowed.as<unsigned>() + (size_t)rows[i] * n, allowed + i * n, n * sizeof(unsigned), cudaMemcpyHostToDevice, stream_));
+    LLM_CUDA(cudaStreamSynchronize(stream_));        // `allowed` has been read
+  }
   if (fresh) {
     // First use: the step runs once outside capture (which also sets kernel attributes and sizes
     // the arena) and its results are this call's results; then the same launches are captured,

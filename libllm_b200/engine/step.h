@@ -38,12 +38,21 @@ struct SamplingParams {
   float temperature = 1.0f;
   int top_k = 50;
   float top_p = 0.8f;
+  // Before the draw (csrc/logits.cu): penalties for the tokens that the sequence holds (Engine::Options::track_history), and numbers that are added to
+  // single tokens' logits, a token at most once.
+  float repetition_penalty = 1.0f, presence_penalty = 0.0f, frequency_penalty = 0.0f;
+  std::vector<std::pair<int, float>> logit_bias;
   void validate() const;
   bool greedy() const { return temperature == 0.f; }
+  bool penalizes() const { return repetition_penalty != 1.f || presence_penalty != 0.f || frequency_penalty != 0.f; }
   bool operator<(const SamplingParams &o) const {
     if (temperature != o.temperature) return temperature < o.temperature;
     if (top_k != o.top_k) return top_k < o.top_k;
-    return top_p < o.top_p;
+    if (top_p != o.top_p) return top_p < o.top_p;
+    if (repetition_penalty != o.repetition_penalty) return repetition_penalty < o.repetition_penalty;
+    if (presence_penalty != o.presence_penalty) return presence_penalty < o.presence_penalty;
+    if (frequency_penalty != o.frequency_penalty) return frequency_penalty < o.frequency_penalty;
+    return logit_bias.empty() && !o.logit_bias.empty();      // the numbers themselves lie in device memory, not in a graph
   }
 };
 
@@ -84,6 +93,7 @@ class Engine {
     int max_step_tokens = 8192;      // a step with more tokens is cut into pieces of this many
     int page_size = 64;
     bool use_graphs = true;
+    bool track_history = false;      // keep every sequence's tokens on the device, for the penalties of SamplingParams: 4 bytes x slots x max_seq_len
     int device = 0;
   };
   Engine(std::unique_ptr<Model> model, const Options &options);
@@ -106,8 +116,11 @@ class Engine {
 
   // Runs the items' tokens.  Without `sampling` the result holds the logits at the wanted places.
   // With it, a token is drawn at each wanted place; `uniforms` then holds one number in [0, 1) per
-  // wanted place (null: zeros).  Returns when the work is queued on the engine's stream.
-  StepResult step(const std::vector<StepItem> &items, const SamplingParams *sampling = nullptr, const float *uniforms = nullptr);
+  // wanted place (null: zeros).  Returns when the work is queued on the engine's stream.  `allowed` (with sampling; null: all): per
+  // wanted place (vocab + 31) / 32 words of host memory, read before the call returns, whose bit v % 32 of word v / 32 says whether token v may be
+  // drawn.  The result's logits are the model's own, without penalties, bias or mask.
+  StepResult step(const std::vector<StepItem> &items, const SamplingParams *sampling = nullptr, const float *uniforms = nullptr,
+                  const uint32_t *allowed = nullptr);
   // Copies a step's logits and tokens (either may be null) to host memory, waits once, and checks the status word.
   void read(const StepResult &r, float *logits, int *tokens);
   // Where results for the host may lie so that the copy engine writes them directly.
@@ -142,19 +155,22 @@ class Engine {
   struct DecodeGraph;
   struct GraphKey {
     int batch, width;
-    bool sampled;
+    bool sampled, masked;
     SamplingParams sampling;
     bool operator<(const GraphKey &o) const;
   };
 
   void validate(const std::vector<StepItem> &items) const;
+  void validate_adjustments(const std::vector<StepItem> &items, const SamplingParams &s) const;
   void fill(Descriptor &d, const std::vector<Piece> &pieces, const std::vector<StepItem> &items, const std::vector<int> &want_rows,
             const float *uniforms, int n_uniforms);
+  void place_history(Descriptor &d);
+  void bring_bias(const SamplingParams &s);
   StepContext context(Descriptor &d, const std::vector<Piece> &pieces, int n_want, bool decode_only, int max_kv_len, Arena *arena,
                       std::vector<const int *> *tables);
-  void sample(const Act &logits, const SamplingParams &s, const float *uniforms_dev, int *out);
-  StepResult run_eager(const std::vector<StepItem> &items, const SamplingParams *sampling, const float *uniforms);
-  StepResult run_decode_graph(const std::vector<StepItem> &items, const SamplingParams *sampling, const float *uniforms);
+  void sample(const Act &logits, const SamplingParams &s, Descriptor &d, const unsigned *allowed_dev, Arena *arena, int *out);
+  StepResult run_eager(const std::vector<StepItem> &items, const SamplingParams *sampling, const float *uniforms, const uint32_t *allowed);
+  StepResult run_decode_graph(const std::vector<StepItem> &items, const SamplingParams *sampling, const float *uniforms, const uint32_t *allowed);
   Act graph_body(DecodeGraph &g);
   void raise_status(int code);
 
@@ -166,6 +182,10 @@ class Engine {
   int sm_count_ = 148;
   Arena scratch_, results_, layer_scratch_[2];
   DeviceBuffer status_, counters_, last_tokens_;
+  DeviceBuffer history_;             // [slots, max_seq_len] (csrc/logits.cu) with Options::track_history
+  int history_places_ = 0;
+  DeviceBuffer bias_;                // [vocab], made when a step first has a bias: the one of the last such step
+  std::vector<std::pair<int, float>> bias_now_;
   std::unique_ptr<Chain> chain_;     // the queue of the step being launched (parts/chain.h)
   int last_capacity_ = 0;
   std::vector<std::unique_ptr<Descriptor>> eager_desc_;

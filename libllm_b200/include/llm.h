@@ -62,13 +62,19 @@ int32_t llm_model_destroy(llm_model_t *m);
 /* kwargs: "filename" (the model folder: config.json and model.safetensors), "device" ("auto" |
  * "cuda"; "cpu" is refused), and, ours: "dtype" ("bfloat16" | "float32"), "max_tokens" (tokens the
  * cache holds), "max_seq_len", "max_slots", "max_step_tokens", "use_graphs", "cuda_device",
- * "strict" (false: tensors that no part asks for are a warning); or, instead of "filename",
+ * "strict" (false: tensors that no part asks for are a warning), "head" ("nvfp4" | "mxfp4": the output
+ * matrix and the rows it meets are brought into four bits), "track_history" (true: the device keeps every
+ * sequence's tokens, which penalties need); or, instead of "filename",
  * "random": {"config": {...}, "seed": n} for random weights drawn on the device. */
 int32_t llm_model_load(llm_model_t *m, llm_json_t *kwargs);
 int32_t llm_model_get_info(llm_model_t *m, llm_json_t *info);
 /* kwargs: "temperature", "top_k", "top_p" (the reference's, with its defaults 1.0 / 50 / 0.8),
  * "prompt_ids" (where the reference has "messages"), and ours: "max_new_tokens", "seed",
- * "stop_token_ids". */
+ * "stop_token_ids", and what is done to the logits before the draw: "repetition_penalty" (1: none; a
+ * token that the sequence holds has its logit divided by it where positive, multiplied elsewhere),
+ * "presence_penalty", "frequency_penalty" (0: none; a token that was drawn n > 0 times loses presence +
+ * n frequency; what a prompt brought does not count), "logit_bias" [[token id, number], ...] (added).
+ * Penalties need a model that was loaded with "track_history". */
 int32_t llm_model_complete(llm_model_t *m, llm_json_t *kwargs, llm_completion_t *comp);
 int32_t llm_completion_init(llm_completion_t *c);
 int32_t llm_completion_destroy(llm_completion_t *c);
@@ -80,8 +86,8 @@ int32_t llm_model_load_tensors(llm_model_t *m, llm_json_t *kwargs, int32_t n, co
                                const int64_t *const *shapes, const int32_t *ndims, const void *const *data);
 
 /* ---- ours: batched generation.  kwargs: "prompts" [[ids]], "max_new_tokens" (a number or one per
- * prompt), "temperature" (0: greedy), "top_k", "top_p", "seed", "stop_token_ids" (absent: the
- * model's own), "max_batch".  result: {"tokens": [[ids]]}.  on_token may be null. */
+ * prompt), "temperature" (0: greedy), "top_k", "top_p", penalties and "logit_bias" as llm_model_complete, "seed",
+ * "stop_token_ids" (absent: the model's own), "max_batch".  result: {"tokens": [[ids]]}.  on_token may be null. */
 typedef void (*llm_token_fn_t)(int32_t request, int32_t token, void *user);
 int32_t llm_model_generate(llm_model_t *m, llm_json_t *kwargs, llm_token_fn_t on_token, void *user, llm_json_t *result);
 
@@ -93,12 +99,20 @@ int32_t llm_model_sequence_length(llm_model_t *m, int32_t slot, int32_t *length)
  * one after another in `tokens`) and wanting n_want[i] places among them (in `want`, relative to
  * the item's tokens).  fed_rows may be null; fed_rows[i] >= 0 makes item i's one token the one
  * the last sampled step drew for that row.  Without sampling (sampling_json null) `logits`
- * receives [sum n_want, vocab] 32-bit values.  With it ({"temperature", "top_k", "top_p"}),
+ * receives [sum n_want, vocab] 32-bit values.  With it ({"temperature", "top_k", "top_p"}, penalties and "logit_bias" as
+ * llm_model_complete; with penalties only an item's last place may be wanted),
  * `sampled` receives a token per wanted place drawn with uniforms[place] in [0, 1) (null: zeros),
- * and `logits`, if not null, the logits as well.  Returns when the results are in host memory. */
+ * and `logits`, if not null, the model's logits as well (without penalties, bias or mask).  Returns when the
+ * results are in host memory.  For the penalties a token counts as drawn when the step before drew it for the
+ * sequence, whether it comes back by its row or by its id; every other token that a step brings counts as a prompt's. */
 int32_t llm_model_step(llm_model_t *m, int32_t n_items, const int32_t *slots, const int32_t *n_tokens, const int32_t *tokens,
                        const int32_t *fed_rows, const int32_t *n_want, const int32_t *want, const char *sampling_json,
                        const float *uniforms, float *logits, int32_t *sampled);
+/* The same with a mask: (vocab + 31) / 32 words per wanted place, whose bit v % 32 of word v / 32 says whether token v may be drawn
+ * (null: all may).  A place whose mask allows nothing draws a valid but meaningless id. */
+int32_t llm_model_step_allowed(llm_model_t *m, int32_t n_items, const int32_t *slots, const int32_t *n_tokens, const int32_t *tokens,
+                               const int32_t *fed_rows, const int32_t *n_want, const int32_t *want, const char *sampling_json,
+                               const float *uniforms, const uint32_t *allowed, float *logits, int32_t *sampled);
 /* A block of page-locked host memory that `logits` may point to: the copy then needs no staging and meets no page fault.  `block` and
  * `data` are null where the model has none left; ordinary memory does as well.  The block stays valid until it is destroyed, also
  * beyond the model's life, and may be destroyed by any thread. */
