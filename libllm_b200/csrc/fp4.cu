@@ -480,6 +480,17 @@ __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
+// A sum times its two rows' scales.  Between 2^-63 and 2^63 (`near_one`) either order is safe: sums lie between 2^-20 and 2^40.  Beyond, scales at
+// opposite ends of the range meet first (their product is in range where one step would leave it), scales at the same end one after the other.
+__device__ __forceinline__ bool near_one(float scale) {
+  const unsigned e = __float_as_uint(scale) >> 23;       // a NaN or a sign is not near
+  return e >= 64 && e <= 190;
+}
+__device__ __forceinline__ float scaled_far(float v, float rw, float rx) {
+  const float p = rw * rx;
+  return fabsf(p) >= 1.17549435e-38f && fabsf(p) <= 3.40282347e38f ? v * p : v * rw * rx;
+}
+
 struct Fp4In {
   const unsigned char *x_scales, *w_scales;
   const float *x_row, *w_row;
@@ -530,6 +541,7 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
   const int kb0 = n_stages * part / parts, kb1 = n_stages * (part + 1) / parts;
   const long long sf_row_tile = (long long)n_stages * S::SF_BYTES;        // bytes of 128 rows' scales
 
+  bool near = true;                            // of the epilogue's tile: scales that may be applied one by one
   if (warp == 0) {
     // ------------------------------------------------------------ loader
     const bool leader = elect_one();
@@ -641,7 +653,14 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
       const float rw = f < N ? in.w_row[f] : 0.f;
       float *rx = row_raw + (warp - 2) * TN;
       __syncwarp();
-      for (int i = lane; i < TN; i += 32) rx[i] = tok0 + i < M ? in.x_row[tok0 + i] : 0.f;
+      near = near_one(rw) || f >= N;
+      for (int i = lane; i < TN; i += 32) {
+        const float r = tok0 + i < M ? in.x_row[tok0 + i] : 1.f;
+        near = near && near_one(r);
+        rx[i] = r;
+      }
+      near = __all_sync(0xffffffffu, near);
+      const float rw1 = near ? rw : 1.f;
       __syncwarp();
       if (!__all_sync(0xffffffffu, mbar_wait(bar_tfull + 8 * acc, (iter >> 1) & 1, abort_flag, status, 4))) break;
       tc_fence_after();
@@ -653,11 +672,18 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
 #pragma unroll
         for (int i = 0; i < 16; i += 4) *reinterpret_cast<float4 *>(r + i) = *reinterpret_cast<const float4 *>(rx + c0 + i);
         tc_ld16(tmem_base + ((unsigned)(quarter * 32) << 16) + (unsigned)(acc * TN + c0), v);
+        if (!near) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            v[i] = scaled_far(v[i], rw, r[i]);
+            r[i] = 1.f;
+          }
+        }
         if (f < N) {
           TO *p = out + (size_t)(tok0 + c0) * ldo + f;
 #pragma unroll
           for (int i = 0; i < 16; ++i, p += ldo)
-            if (i < n) *p = from_float<TO>(v[i] * rw * r[i]);
+            if (i < n) *p = from_float<TO>(v[i] * rw1 * r[i]);
         }
       }
       tc_fence_before();
@@ -676,7 +702,7 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
     if (warp >= 2) {
       const unsigned mine = smem_u32(smem) + ((unsigned)(part * share) * FP_ROWS + (unsigned)row) * 4;      // of my part, in whosever ring
       float v[2][16];
-#pragma unroll
+#pragma unroll 1
       for (int c0 = 0; c0 < TN; c0 += 32) {
         const unsigned taddr = tmem_base + ((unsigned)(quarter * 32) << 16) + (unsigned)c0;
         tc_ld16(taddr, v[0]);
@@ -698,7 +724,7 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
 #pragma unroll
         for (int q = 0; q < 8; ++q)
           if (q < parts) v += sums[(q * share + c) * FP_ROWS];
-        *p = from_float<TO>(v * rw * rx[c]);
+        *p = from_float<TO>(near ? v * rw * rx[c] : scaled_far(v, rw, rx[c]));
       }
     }
   }
@@ -786,18 +812,18 @@ int launch_fp4(const void *x_codes, const void *w_codes, const Fp4In &in, void *
 // features.  The epilogue warps scale the sums, put boxes of 32 x 32 into buffers of their own, two in turn, and have TMA store them.  A result
 // whose rows do not start on 16 bytes, and the box that hangs over the last feature, are stored by the lanes themselves.
 constexpr int PR_TOKENS = 256, PR_FEATURES = 192;
-constexpr int PR_WARPS = 8;                    // of the epilogue: two to a quarter of the lanes, 96 features each
-constexpr int PR_THREADS = 64 + 32 * PR_WARPS;
 template <int FORMAT, typename TO>
 struct PairShape {
   static constexpr int TILES = stage_tiles(FORMAT), SF_BYTES = TILES * SF_TILE;
   static constexpr int A_BYTES = PR_TOKENS / 2 * 128, B_BYTES = PR_FEATURES / 2 * 128;
   static constexpr int STAGE_BYTES = A_BYTES + B_BYTES + 3 * SF_BYTES;
   static constexpr int STAGES = sizeof(TO) == 4 ? 4 : 5;
+  static constexpr int SHARES = sizeof(TO) == 4 ? 2 : 3, SHARE = PR_FEATURES / SHARES;    // epilogue warps to a quarter of the lanes; their features
+  static constexpr int WARPS = 4 * SHARES, THREADS = 64 + 32 * WARPS;
   static constexpr int SF_COLS = TILES * 12;                             // columns of a stage's scales: 4 of a tile for the tokens, 8 for the features
   static constexpr int OUT_BYTES = 32 * 32 * (int)sizeof(TO);            // 32 tokens x 32 features on their way out
-  static constexpr int ROW_BYTES = PR_WARPS * PR_FEATURES / 2 * 4;       // row scales of its features, for each epilogue warp
-  static constexpr size_t SMEM = 1024 + (size_t)STAGES * STAGE_BYTES + 2 * PR_WARPS * OUT_BYTES + ROW_BYTES + 256;
+  static constexpr int ROW_BYTES = WARPS * SHARE * 4;       // row scales of its features, for each epilogue warp
+  static constexpr size_t SMEM = 1024 + (size_t)STAGES * STAGE_BYTES + 2 * WARPS * OUT_BYTES + ROW_BYTES + 256;
   static_assert(STAGE_BYTES % 1024 == 0 && 2 * PR_FEATURES + 2 * SF_COLS <= 512, "a stage's parts do not fit");
 };
 __device__ __forceinline__ void pair_load(unsigned dst, const CUtensorMap *map, int x, int y, unsigned bar) {
@@ -848,7 +874,7 @@ __device__ __forceinline__ void put16(unsigned box, int row, int half, const flo
 }
 
 template <int FORMAT, typename TO>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PR_THREADS, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__((PairShape<FORMAT, TO>::THREADS), 1)
 fp4_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_xs,
                 const __grid_constant__ CUtensorMap map_ws, const __grid_constant__ CUtensorMap map_out, const float *x_row, const float *w_row, TO *out,
                 long long ldo, int M, int N, int n_stages, int tok_tiles, int feature_tiles, int weights_first, int by_tma, int *status) {
@@ -857,7 +883,7 @@ fp4_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
   extern __shared__ unsigned char smem_raw[];
   unsigned char *smem = (unsigned char *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   unsigned char *out_raw = smem + (size_t)STAGES * S::STAGE_BYTES;
-  float *row_raw = (float *)(out_raw + 2 * PR_WARPS * S::OUT_BYTES);
+  float *row_raw = (float *)(out_raw + 2 * S::WARPS * S::OUT_BYTES);
   unsigned long long *bars = (unsigned long long *)((unsigned char *)row_raw + S::ROW_BYTES);
   const unsigned bar_full = smem_u32(bars), bar_empty = smem_u32(bars + STAGES);
   const unsigned bar_tfull = smem_u32(bars + 2 * STAGES), bar_tempty = smem_u32(bars + 2 * STAGES + 2);
@@ -873,7 +899,7 @@ fp4_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
     }
     for (int a = 0; a < 2; ++a) {
       mbar_init(bar_tfull + 8 * a, 1);         // each CTA's own
-      mbar_init(bar_tempty + 8 * a, 2 * PR_WARPS);      // rank 0's: the epilogue warps of both
+      mbar_init(bar_tempty + 8 * a, 2 * S::WARPS);      // rank 0's: the epilogue warps of both
     }
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -998,27 +1024,33 @@ fp4_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
     }
     grid_dependency_wait();
   } else {
-    // ------------------------------------------------------------ epilogue of this CTA's 128 tokens (warps 2..9)
+    // ------------------------------------------------------------ epilogue of this CTA's 128 tokens (warps 2 and up)
     grid_dependency_wait();
-    const int quarter = warp & 3, half = (warp - 2) / 4;       // the lanes of tensor memory the warp may read; its half of the features
+    const int quarter = warp & 3, from = (warp - 2) / 4 * S::SHARE;        // the lanes of tensor memory the warp may read; its first feature
     const unsigned box0 = smem_u32(out_raw) + (unsigned)(warp - 2) * 2 * S::OUT_BYTES;
-    float *rows = row_raw + (warp - 2) * (PR_FEATURES / 2);
+    float *rows = row_raw + (warp - 2) * S::SHARE;
     int iter = 0;
     unsigned turn = 0;
     for (int tile = first; tile < n_tiles; tile += step, ++iter) {
-      const int acc = iter & 1, f0 = tile / tok_tiles * PR_FEATURES + half * (PR_FEATURES / 2);
+      const int acc = iter & 1, f0 = tile / tok_tiles * PR_FEATURES + from;
       const int tok0 = tile % tok_tiles * PR_TOKENS + (int)rank * 128 + quarter * 32;
       // the rows' scales, while the products run: from memory at each use they cost more than the rest of the epilogue
       const float rx = tok0 + lane < M ? x_row[tok0 + lane] : 0.f;
       __syncwarp();
+      bool near = near_one(rx) || tok0 + lane >= M;
 #pragma unroll
-      for (int i = lane; i < PR_FEATURES / 2; i += 32) rows[i] = f0 + i < N ? w_row[f0 + i] : 0.f;
+      for (int i = lane; i < S::SHARE; i += 32) {
+        const float r = f0 + i < N ? w_row[f0 + i] : 1.f;
+        near = near && near_one(r);
+        rows[i] = r;
+      }
+      near = __all_sync(0xffffffffu, near);
       __syncwarp();
       if (!__all_sync(0xffffffffu, mbar_wait(bar_tfull + 8 * acc, (iter >> 1) & 1, abort_flag, status, 4))) break;
       tc_fence_after();
-      const unsigned taddr = tmem_base + ((unsigned)(quarter * 32) << 16) + (unsigned)(acc * PR_FEATURES + half * (PR_FEATURES / 2));
+      const unsigned taddr = tmem_base + ((unsigned)(quarter * 32) << 16) + (unsigned)(acc * PR_FEATURES + from);
 #pragma unroll 1
-      for (int s0 = 0; s0 < PR_FEATURES / 2 && f0 + s0 < N && tok0 < M; s0 += 32, turn ^= 1) {
+      for (int s0 = 0; s0 < S::SHARE && f0 + s0 < N && tok0 < M; s0 += 32, turn ^= 1) {
         const unsigned box = box0 + turn * S::OUT_BYTES;
         float a[16], b[16];
         tc_ld16_issue(taddr + s0, a);
@@ -1026,17 +1058,25 @@ fp4_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
         tc_ld_wait();
         tc_ld_ready(a);
         tc_ld_ready(b);
+        if (near) {
 #pragma unroll
-        for (int i = 0; i < 16; i += 4) {
-          const float4 r = *reinterpret_cast<const float4 *>(rows + s0 + i), q = *reinterpret_cast<const float4 *>(rows + s0 + 16 + i);
-          a[i] = a[i] * r.x * rx;
-          a[i + 1] = a[i + 1] * r.y * rx;
-          a[i + 2] = a[i + 2] * r.z * rx;
-          a[i + 3] = a[i + 3] * r.w * rx;
-          b[i] = b[i] * q.x * rx;
-          b[i + 1] = b[i + 1] * q.y * rx;
-          b[i + 2] = b[i + 2] * q.z * rx;
-          b[i + 3] = b[i + 3] * q.w * rx;
+          for (int i = 0; i < 16; i += 4) {
+            const float4 r = *reinterpret_cast<const float4 *>(rows + s0 + i), q = *reinterpret_cast<const float4 *>(rows + s0 + 16 + i);
+            a[i] = a[i] * r.x * rx;
+            a[i + 1] = a[i + 1] * r.y * rx;
+            a[i + 2] = a[i + 2] * r.z * rx;
+            a[i + 3] = a[i + 3] * r.w * rx;
+            b[i] = b[i] * q.x * rx;
+            b[i + 1] = b[i + 1] * q.y * rx;
+            b[i + 2] = b[i + 2] * q.z * rx;
+            b[i + 3] = b[i + 3] * q.w * rx;
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            a[i] = scaled_far(a[i], rows[s0 + i], rx);
+            b[i] = scaled_far(b[i], rows[s0 + 16 + i], rx);
+          }
         }
         // what hangs over the last column is stored lane by lane: TMA would round its end up to 16 bytes, into what is not ours
         if (by_tma && f0 + s0 + 32 <= N) {
@@ -1128,7 +1168,7 @@ int launch_pair(const void *x_codes, const void *w_codes, const Fp4In &in, void 
   const int pairs = (int)(tiles < sm_count() / 2 ? tiles : sm_count() / 2);
   auto kern = fp4_pair_kernel<FORMAT, TO>;
   LLM_CHECK_CUDA(llm_allow_smem(kern, S::SMEM), "fp4_gemm attribute");
-  LLM_CHECK_CUDA(llm_launch(kern, dim3(2 * pairs), dim3(PR_THREADS), S::SMEM, stream, map_x, map_w, map_xs, map_ws, map_out, in.x_row, in.w_row, (TO *)out,
+  LLM_CHECK_CUDA(llm_launch(kern, dim3(2 * pairs), dim3(S::THREADS), S::SMEM, stream, map_x, map_w, map_xs, map_ws, map_out, in.x_row, in.w_row, (TO *)out,
                             ldo, M, N, (int)k_stages(K), tok_tiles, feature_tiles, weights_first, by_tma ? 1 : 0, status),
                  "fp4_gemm launch");
   return LLM_OK;

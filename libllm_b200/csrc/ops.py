@@ -367,14 +367,18 @@ _current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device
 
 def _same_device(first: torch.Tensor, *others) -> int:
     """The tensors lie on the current device, where the launch goes; its current stream's handle."""
-    if not first.is_cuda:
-        _on_gpu(first)
-    current = _current_device()
-    for t in (first, *others):
+    current = first.get_device()
+    if current < 0 or current != _current_device():
+        _other_device(first)
+    for t in others:
         if t is not None and t.get_device() != current:
-            _on_gpu(t)
-            raise InvalidArgError(f"a tensor lies on '{t.device}', the launch goes to the current device 'cuda:{current}'")
+            _other_device(t)
     return _raw_stream(current) if _raw_stream is not None else torch.cuda.current_stream().cuda_stream
+
+
+def _other_device(t: torch.Tensor) -> None:
+    _on_gpu(t)
+    raise InvalidArgError(f"a tensor lies on '{t.device}', the launch goes to the current device 'cuda:{torch.cuda.current_device()}'")
 
 
 def _per_row(name: str, v, rows: int, *, positive: bool = False):
@@ -533,37 +537,46 @@ def fp4_quantize(x: torch.Tensor, format: str = "nvfp4", out: Optional[Fp4Matrix
     """x [rows, cols] (bfloat16 or float32, any row stride) in four bits.  nvfp4: blocks of 16 along a row with e4m3 scales and a power of two
     per row; mxfp4: blocks of 32 with powers of two.  A code is the nearest one, halves go to the even code, what is too large becomes the
     largest.  A row that holds a NaN or an infinity becomes NaN throughout.  ``out``: a matrix of the same shape and format to fill."""
-    if x.dim() != 2 or (x.shape[1] > 1 and x.stride(1) != 1):
-        raise InvalidArgError("fp4_quantize: x is [rows, cols] with neighbouring columns")
-    dt = dtype_code(x.dtype)
-    rows, cols = x.shape
+    shape, dt = x.shape, _DT.get(x.dtype)
+    if len(shape) != 2:
+        raise InvalidArgError("fp4_quantize: x is [rows, cols]")
+    rows, cols = shape
+    ld, step = x.stride()
+    if step != 1 and cols > 1:
+        raise InvalidArgError("fp4_quantize: the values of a row are neighbours")
+    if dt is None:
+        dtype_code(x.dtype)                     # says which are taken
     if out is None:
         if (rows, cols, format) not in _fp4_layouts:
             _fp4_layout(rows, cols, format)
         stream = _same_device(x)
         out = Fp4Matrix(rows, cols, format, x.device)
     else:
-        if (out.rows, out.cols, out.format) != (rows, cols, format):
+        if out.rows != rows or out.cols != cols or out.format != format:
             raise InvalidArgError(f"fp4_quantize: out is {out.format} [{out.rows}, {out.cols}], x becomes {format} [{rows}, {cols}]")
         stream = _same_device(x, out.data)
     number, _, scales, row, _ = out._layout
     p = out.data.data_ptr()
-    _call_packed("fp4", "llm_fp4_quantize", _pack_fp4_quantize(dt, x.data_ptr(), x.stride(0), p, p + scales, p + row, rows, cols, number, stream))
+    _call_packed("fp4", "llm_fp4_quantize", _pack_fp4_quantize(dt, x.data_ptr(), ld, p, p + scales, p + row, rows, cols, number, stream))
     return out
 
 
 def fp4_dequantize(q: Fp4Matrix, dtype: torch.dtype = torch.float32, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """What a matrix in four bits stands for, [rows, cols] float32 or bfloat16 (both hold it exactly where it is within
     their range; an nvfp4 scale that was rounded up may take a value within 3 % of the largest number beyond it)."""
-    dt = dtype_code(dtype if out is None else out.dtype)
-    if out is not None and (out.shape != (q.rows, q.cols) or (q.cols > 1 and out.stride(1) != 1) or (q.rows > 1 and out.stride(0) < q.cols)):
-        raise InvalidArgError(f"fp4_dequantize: out is [{q.rows}, {q.cols}] with neighbouring columns and rows of its own")
-    stream = _same_device(q.data, out)
+    dt, rows, cols = dtype_code(dtype if out is None else out.dtype), q.rows, q.cols
     if out is None:
-        out = torch.empty(q.rows, q.cols, dtype=dtype, device=q.data.device)
+        ldo = cols
+        stream = _same_device(q.data)
+        out = torch.empty(rows, cols, dtype=dtype, device=q.data.device)
+    else:
+        if out.shape != (rows, cols) or (cols > 1 and out.stride(1) != 1) or (rows > 1 and out.stride(0) < cols):
+            raise InvalidArgError(f"fp4_dequantize: out is [{rows}, {cols}] with neighbouring columns and rows of its own")
+        ldo = out.stride(0)
+        stream = _same_device(q.data, out)
     number, _, scales, row, _ = q._layout
     p = q.data.data_ptr()
-    _call_packed("fp4", "llm_fp4_dequantize", _pack_fp4_dequantize(p, p + scales, p + row, dt, out.data_ptr(), out.stride(0), q.rows, q.cols, number, stream))
+    _call_packed("fp4", "llm_fp4_dequantize", _pack_fp4_dequantize(p, p + scales, p + row, dt, out.data_ptr(), ldo, rows, cols, number, stream))
     return out
 
 
@@ -573,19 +586,25 @@ def fp4_gemm(x: Fp4Matrix, w: Fp4Matrix, out: Optional[torch.Tensor] = None, out
     if x.format != w.format or x.cols != w.cols:
         raise InvalidArgError(f"fp4_gemm: {x.format} [{x.rows}, {x.cols}] and {w.format} [{w.rows}, {w.cols}] do not meet")
     M, N = x.rows, w.rows
-    if max(M, N) >= 1 << 30:
+    if M >= 1 << 30 or N >= 1 << 30:
         raise UnsupportedError(f"fp4_gemm: {M} x {N} is not taken")
-    dt = dtype_code(out_dtype if out is None else out.dtype)
-    if out is not None and (out.shape != (M, N) or (N > 1 and out.stride(1) != 1) or (M > 1 and out.stride(0) < N)):
-        raise InvalidArgError(f"fp4_gemm: out is [{M}, {N}] with neighbouring columns and rows of its own")
-    stream = _same_device(x.data, w.data, out)
+    xd, wd = x.data, w.data
     if out is None:
-        out = torch.empty(M, N, dtype=out_dtype, device=w.data.device)
+        dt = dtype_code(out_dtype)
+        stream = _same_device(wd, xd)
+        ldo = N
+        out = torch.empty(M, N, dtype=out_dtype, device=wd.device)
+    else:
+        dt = dtype_code(out.dtype)
+        if out.shape != (M, N) or (N > 1 and out.stride(1) != 1) or (M > 1 and out.stride(0) < N):
+            raise InvalidArgError(f"fp4_gemm: out is [{M}, {N}] with neighbouring columns and rows of its own")
+        stream = _same_device(wd, xd, out)
+        ldo = out.stride(0)
     number, _, xs, xr, _ = x._layout
     _, _, ws, wr, _ = w._layout
-    xp, wp = x.data.data_ptr(), w.data.data_ptr()
-    _call_packed("fp4", "llm_fp4_gemm", _pack_fp4_gemm(xp, xp + xs, xp + xr, wp, wp + ws, wp + wr, dt, out.data_ptr(), out.stride(0), M, N, x.cols, number, 0,
-                                                       _status_word(w.data.device), stream))
+    xp, wp = xd.data_ptr(), wd.data_ptr()
+    _call_packed("fp4", "llm_fp4_gemm", _pack_fp4_gemm(xp, xp + xs, xp + xr, wp, wp + ws, wp + wr, dt, out.data_ptr(), ldo, M, N, x.cols, number, 0,
+                                                       _status_words.get(wd.get_device()) or _status_word(wd.device), stream))
     return out
 
 

@@ -205,6 +205,22 @@ def test_a_tokens_result_does_not_hang_on_the_others(format):
         assert torch.equal(o.fp4_gemm(o.fp4_quantize(x[:n], format), qw), whole[:n])
 
 
+@pytest.mark.parametrize("M", [5, 100, 400])
+@pytest.mark.parametrize("up,down", [(120, -120), (-120, 120), (126, -126), (55, 55), (-60, -60), (-70, -50), (100, -30), (-124, 0)])
+def test_rows_at_the_ends_of_the_range(M, up, down):
+    """Scales at opposite ends of the range cancel; at the same end what can be held is held (terms of 2^-20 and more, 2^40 at most)."""
+    o = ops()
+    K, N = 300, 150
+    x, w = rows_like(M, K, 1, spread=1).double() * 2.0 ** up, rows_like(N, K, 2, spread=1).double() * 2.0 ** down
+    x, w = (x.clamp(-3e38, 3e38).to(torch.bfloat16), w.clamp(-3e38, 3e38).to(torch.bfloat16))
+    got = o.fp4_gemm(o.fp4_quantize(x.to(DEV)), o.fp4_quantize(w.to(DEV))).double().cpu()
+    o.check_tc_status()
+    a, b = P.values(x, "nvfp4"), P.values(w, "nvfp4")
+    ref, size = a @ b.T, a.abs() @ b.abs().T
+    tol = size * (K + 2) * 2.0 ** -23 + 2.0 ** -149
+    assert ((got - ref).abs() <= tol).all(), f"worst {float(((got - ref).abs() / tol).max()):.2f} of what is allowed"
+
+
 def test_nothing_to_do():
     o = ops()
     none = o.fp4_quantize(torch.empty(0, 64, dtype=torch.bfloat16, device=DEV))
