@@ -1,9 +1,11 @@
 """Builds the native code of this package and loads it with ctypes.
 
-Two kinds of things are built, each the first time something needs it:
+Three kinds of things are built, each the first time something needs it:
 
 * the **kernel families**: every ``.cu`` of this folder is one shared library for sm_100a,
   compiled by nvcc; a model compiles the families that its type, head size and grouping use;
+* the **torch binding** of the calls whose arguments would take longer than their kernels
+  (``torch_calls.cpp``), compiled by g++ against torch's headers;
 * the **host library** ``libllm_b200`` (configuration, weights, cache, step function, generation
   loop, C interface: the ``.cc`` files of the package) and the ``llm`` program, compiled by g++
   and linked against the CUDA runtime.
@@ -350,6 +352,66 @@ def build_cli() -> str:
     os.replace(tmp, out)
     _remove_older("llm-", out)
     return out
+
+
+# ---------------------------------------------------------------- the torch binding
+_BINDING_SOURCES = ["torch_calls.cpp", "fp4.h", "logits.h"]
+_BINDING_FLAGS = ["-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden"]
+
+
+def binding_path() -> str:
+    import sysconfig
+    import torch
+    h = hashlib.sha1()
+    for f in _BINDING_SOURCES:
+        with open(os.path.join(HERE, f), "rb") as fh:
+            h.update(f.encode())
+            h.update(fh.read())
+    h.update(" ".join(_BINDING_FLAGS + [torch.__version__, sysconfig.get_config_var("SOABI") or ""]).encode())
+    return os.path.join(build_dir(), f"libllm_torch_calls-{h.hexdigest()[:12]}.so")
+
+
+def build_binding() -> str:
+    out = binding_path()
+    if os.path.isfile(out):
+        return out
+    import sysconfig
+    import torch
+    base = os.path.dirname(os.path.abspath(torch.__file__))
+    tmp = f"{out}.{os.getpid()}.{threading.get_ident()}.tmp"
+    _say("compiling torch_calls.cpp ...")
+    t0 = time.time()
+    _run([_gxx()] + _BINDING_FLAGS + ["-I", HERE, "-isystem", os.path.join(base, "include"),
+                                      "-isystem", os.path.join(base, "include", "torch", "csrc", "api", "include"),
+                                      "-I", sysconfig.get_paths()["include"], "-I", os.path.join(cuda_home(), "include"), "-o", tmp,
+                                      os.path.join(HERE, _BINDING_SOURCES[0]), "-L", os.path.join(base, "lib"), "-ltorch_python", "-ltorch_cpu", "-lc10",
+                                      "-lc10_cuda"], "torch_calls")
+    os.replace(tmp, out)
+    _remove_older("libllm_torch_calls-", out)
+    _say(f"built {os.path.basename(out)} in {time.time() - t0:.1f} s")
+    return out
+
+
+_binding = None
+
+
+def load_binding():
+    """The module of ``torch_calls.cpp``, built first if need be."""
+    global _binding
+    if _binding is None:
+        with _lock:
+            if _binding is None:
+                import importlib.machinery
+                import importlib.util
+                path = build_binding()
+                loader = importlib.machinery.ExtensionFileLoader("llm_torch_calls", path)
+                try:
+                    module = importlib.util.module_from_spec(importlib.util.spec_from_loader("llm_torch_calls", loader))
+                    loader.exec_module(module)
+                except ImportError as e:
+                    raise ExtensionError(f"cannot load {path}: {e}") from None
+                _binding = module
+    return _binding
 
 
 _host = None

@@ -90,6 +90,27 @@ def _call_packed(family: str, name: str, args: bytes) -> None:
         _raise(name, status, f[1])
 
 
+_quick = {}
+
+
+def _quick_call(family: str, name: str, t: torch.Tensor):
+    """A function of the torch binding (csrc/torch_calls.cpp), tied to its kernel's library, for calls whose first tensor is ``t``.  It answers
+    None to a call that is not plainly right: the checks here then say what is wrong with it."""
+    if not t.is_cuda:
+        return lambda *args: None
+    binding = build.load_binding()
+    binding.bind("llm_" + name, ctypes.cast(_fn(family, "llm_" + name, [c_char_p])[0], c_void_p).value)
+    f = _quick[name] = getattr(binding, name)
+    return f
+
+
+def _launched(family: str, name: str, result) -> None:
+    """A quick call's answer is a tensor, or the status that the kernel's library refused with."""
+    LAUNCHES[0] += 1
+    if type(result) is int:
+        _raise("llm_" + name, result, _fn(family, "llm_" + name, [c_char_p])[1])
+
+
 def _raise(name: str, status: int, err) -> None:
     msg = err().decode("utf-8", "replace")
     if status == 0x0100:
@@ -409,6 +430,11 @@ def adjust_logits(logits: torch.Tensor, out: Optional[torch.Tensor] = None, hist
     itself without slots; a place outside the history: an empty one), an id for a token that was drawn, ~id for one that a prompt brought; ids
     outside the vocabulary count for nothing.  repetition (above 0), presence and frequency: a number, or a float32 tensor [B]; without a
     history they do nothing.  ``out`` (new where None) may be ``logits`` itself, and no other tensor that overlaps it.  All 32-bit."""
+    result = (_quick.get("adjust_logits") or _quick_call("logits", "adjust_logits", logits))(
+        logits, out, history, slots, lengths, repetition, presence, frequency, bias, allowed)
+    if result is not None:
+        _launched("logits", "adjust_logits", result)
+        return result
     if logits.dim() != 2 or logits.dtype != _F32:
         raise InvalidArgError("adjust_logits: logits are float32 [rows, vocabulary]")
     B, V = logits.shape
@@ -494,6 +520,16 @@ class Fp4Matrix:
         self.format = format
         self.data = torch.empty(layout[4], dtype=torch.uint8, device=device)
 
+    @classmethod
+    def _of(cls, data: torch.Tensor, rows: int, cols: int, format: str) -> "Fp4Matrix":
+        q = cls.__new__(cls)
+        q._layout = _fp4_layouts.get((rows, cols, format)) or _fp4_layout(rows, cols, format)
+        q.rows = rows
+        q.cols = cols
+        q.format = format
+        q.data = data
+        return q
+
     @property
     def device(self):
         return self.data.device
@@ -537,6 +573,11 @@ def fp4_quantize(x: torch.Tensor, format: str = "nvfp4", out: Optional[Fp4Matrix
     """x [rows, cols] (bfloat16 or float32, any row stride) in four bits.  nvfp4: blocks of 16 along a row with e4m3 scales and a power of two
     per row; mxfp4: blocks of 32 with powers of two.  A code is the nearest one, halves go to the even code, what is too large becomes the
     largest.  A row that holds a NaN or an infinity becomes NaN throughout.  ``out``: a matrix of the same shape and format to fill."""
+    if out is None and format in FP4_FORMATS:
+        data = (_quick.get("fp4_quantize") or _quick_call("fp4", "fp4_quantize", x))(x, FP4_FORMATS[format])
+        if data is not None:
+            _launched("fp4", "fp4_quantize", data)
+            return Fp4Matrix._of(data, *x.shape, format)
     shape, dt = x.shape, _DT.get(x.dtype)
     if len(shape) != 2:
         raise InvalidArgError("fp4_quantize: x is [rows, cols]")
@@ -566,6 +607,11 @@ def fp4_dequantize(q: Fp4Matrix, dtype: torch.dtype = torch.float32, out: Option
     their range; an nvfp4 scale that was rounded up may take a value within 3 % of the largest number beyond it)."""
     dt, rows, cols = dtype_code(dtype if out is None else out.dtype), q.rows, q.cols
     if out is None:
+        values = (_quick.get("fp4_dequantize") or _quick_call("fp4", "fp4_dequantize", q.data))(q.data, rows, cols, q._layout[0], dt)
+        if values is not None:
+            _launched("fp4", "fp4_dequantize", values)
+            return values
+    if out is None:
         ldo = cols
         stream = _same_device(q.data)
         out = torch.empty(rows, cols, dtype=dtype, device=q.data.device)
@@ -589,8 +635,14 @@ def fp4_gemm(x: Fp4Matrix, w: Fp4Matrix, out: Optional[torch.Tensor] = None, out
     if M >= 1 << 30 or N >= 1 << 30:
         raise UnsupportedError(f"fp4_gemm: {M} x {N} is not taken")
     xd, wd = x.data, w.data
+    device = wd.get_device()
+    word = 0 if device < 0 else _status_words.get(device) or _status_word(wd.device)
     if out is None:
         dt = dtype_code(out_dtype)
+        result = (_quick.get("fp4_gemm") or _quick_call("fp4", "fp4_gemm", wd))(xd, wd, M, N, x.cols, x._layout[0], dt, word)
+        if result is not None:
+            _launched("fp4", "fp4_gemm", result)
+            return result
         stream = _same_device(wd, xd)
         ldo = N
         out = torch.empty(M, N, dtype=out_dtype, device=wd.device)
@@ -604,7 +656,7 @@ def fp4_gemm(x: Fp4Matrix, w: Fp4Matrix, out: Optional[torch.Tensor] = None, out
     _, _, ws, wr, _ = w._layout
     xp, wp = xd.data_ptr(), wd.data_ptr()
     _call_packed("fp4", "llm_fp4_gemm", _pack_fp4_gemm(xp, xp + xs, xp + xr, wp, wp + ws, wp + wr, dt, out.data_ptr(), ldo, M, N, x.cols, number, 0,
-                                                       _status_words.get(wd.get_device()) or _status_word(wd.device), stream))
+                                                       word, stream))
     return out
 
 
