@@ -28,7 +28,7 @@ namespace {
 
 enum Fp4Format { NVFP4 = 0, MXFP4 = 1 };
 
-constexpr int UNIT = 8;                        // values that a thread brings into four bits at once: 4 bytes of codes
+constexpr int UNIT = 16;                       // values that a thread brings into four bits at once: 8 bytes of codes
 constexpr int STAGE_K = 256;                   // of the product: 128 bytes of codes, one swizzle row
 constexpr int SF_TILE = 512;                   // bytes of scales: 128 rows x 4 blocks
 
@@ -37,69 +37,61 @@ __host__ __device__ inline long long k_stages(long long K) { return (K + STAGE_K
 __host__ __device__ inline long long code_bytes(long long K) { return (K + 31) / 32 * 16; }           // of a row
 
 // ---------------------------------------------------------------- into four bits
-// UNIT values of a row as they lie in memory.  A warp's 32 units are 256 of K: the lanes of a block of nvfp4 are two, of mxfp4 four.
+// UNIT values of a row as they lie in memory, a lane's share: a block of nvfp4, half of one of mxfp4.
 template <typename T>
 struct Unit;
 template <>
 struct Unit<__nv_bfloat16> {
-  unsigned w[4];
+  unsigned w[UNIT / 2];
   __device__ __forceinline__ void load(const __nv_bfloat16 *p) {
-    const uint4 raw = *reinterpret_cast<const uint4 *>(p);
-    w[0] = raw.x;
-    w[1] = raw.y;
-    w[2] = raw.z;
-    w[3] = raw.w;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const uint4 raw = reinterpret_cast<const uint4 *>(p)[i];
+      w[4 * i] = raw.x;
+      w[4 * i + 1] = raw.y;
+      w[4 * i + 2] = raw.z;
+      w[4 * i + 3] = raw.w;
+    }
   }
   __device__ __forceinline__ void gather(const __nv_bfloat16 *p, int n) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < UNIT / 2; ++i) {
       const unsigned lo = 2 * i < n ? __bfloat16_as_ushort(p[2 * i]) : 0, hi = 2 * i + 1 < n ? __bfloat16_as_ushort(p[2 * i + 1]) : 0;
       w[i] = lo | hi << 16;
     }
   }
-  __device__ __forceinline__ void values(float (&v)[UNIT]) const {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      v[2 * i] = __uint_as_float(w[i] << 16);
-      v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-    }
-  }
+  __device__ __forceinline__ float2 two(int i) const { return make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u)); }
   // The largest magnitude's bits, as those of a 32-bit value: as whole numbers they are in the order of the values, and every infinity and NaN is
   // 0x7f800000 or more.
   __device__ __forceinline__ unsigned top() const {
-    const unsigned m = __vmaxu2(__vmaxu2(w[0] & 0x7fff7fffu, w[1] & 0x7fff7fffu), __vmaxu2(w[2] & 0x7fff7fffu, w[3] & 0x7fff7fffu));
+    unsigned m = w[0] & 0x7fff7fffu;
+#pragma unroll
+    for (int i = 1; i < UNIT / 2; ++i) m = __vmaxu2(m, w[i] & 0x7fff7fffu);
     return max(m << 16, m & 0xffff0000u);
   }
 };
 template <>
 struct Unit<float> {
-  float4 raw[2];
+  float4 raw[UNIT / 4];
   __device__ __forceinline__ void load(const float *p) {
-    raw[0] = reinterpret_cast<const float4 *>(p)[0];
-    raw[1] = reinterpret_cast<const float4 *>(p)[1];
+#pragma unroll
+    for (int i = 0; i < UNIT / 4; ++i) raw[i] = reinterpret_cast<const float4 *>(p)[i];
   }
   __device__ __forceinline__ void gather(const float *p, int n) {
     float v[UNIT];
 #pragma unroll
     for (int i = 0; i < UNIT; ++i) v[i] = i < n ? p[i] : 0.f;
-    raw[0] = make_float4(v[0], v[1], v[2], v[3]);
-    raw[1] = make_float4(v[4], v[5], v[6], v[7]);
-  }
-  __device__ __forceinline__ void values(float (&v)[UNIT]) const {
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      v[4 * i] = raw[i].x;
-      v[4 * i + 1] = raw[i].y;
-      v[4 * i + 2] = raw[i].z;
-      v[4 * i + 3] = raw[i].w;
-    }
+    for (int i = 0; i < UNIT / 4; ++i) raw[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
   }
+  __device__ __forceinline__ float2 two(int i) const { return i % 2 ? make_float2(raw[i / 2].z, raw[i / 2].w) : make_float2(raw[i / 2].x, raw[i / 2].y); }
   __device__ __forceinline__ unsigned top() const {
-    float v[UNIT];
-    values(v);
     unsigned m = 0;
 #pragma unroll
-    for (int i = 0; i < UNIT; ++i) m = max(m, __float_as_uint(v[i]) & 0x7fffffffu);
+    for (int i = 0; i < UNIT / 2; ++i) {
+      const float2 v = two(i);
+      m = max(m, max(__float_as_uint(v.x) & 0x7fffffffu, __float_as_uint(v.y) & 0x7fffffffu));
+    }
     return m;
   }
 };
@@ -112,13 +104,34 @@ __device__ __forceinline__ Unit<T> fetch_unit(const T *row, int u, int K, bool v
   return x;
 }
 
-__device__ __forceinline__ unsigned pack_codes(const float (&v)[UNIT]) {      // the first in the lowest four bits
+// Two 32-bit products with a sum, or without, in one instruction.
+__device__ __forceinline__ float2 fma_two(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n.reg .b64 a, b, c, d;\nmov.b64 a, {%2, %3};\nmov.b64 b, {%4, %5};\nmov.b64 c, {%6, %7};\n"
+      "fma.rn.f32x2 d, a, b, c;\nmov.b64 {%0, %1}, d;\n}"
+      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float2 add_two(float2 a, float2 b) {
+  float2 d;
+  asm("{\n.reg .b64 a, b, d;\nmov.b64 a, {%2, %3};\nmov.b64 b, {%4, %5};\nadd.rn.f32x2 d, a, b;\nmov.b64 {%0, %1}, d;\n}"
+      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ float2 mul_two(float2 a, float2 b) {
+  float2 d;
+  asm("{\n.reg .b64 a, b, d;\nmov.b64 a, {%2, %3};\nmov.b64 b, {%4, %5};\nmul.rn.f32x2 d, a, b;\nmov.b64 {%0, %1}, d;\n}"
+      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+
+__device__ __forceinline__ unsigned pack_codes(const float2 *v) {      // eight values, the first in the lowest four bits
   unsigned r;
   asm("{\n.reg .b8 a, b, c, d;\n"
       "cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\ncvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n"
       "cvt.rn.satfinite.e2m1x2.f32 c, %6, %5;\ncvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\n"
       "mov.b32 %0, {a, b, c, d};\n}"
-      : "=r"(r) : "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]));
+      : "=r"(r) : "f"(v[0].x), "f"(v[0].y), "f"(v[1].x), "f"(v[1].y), "f"(v[2].x), "f"(v[2].y), "f"(v[3].x), "f"(v[3].y));
   return r;
 }
 
@@ -130,7 +143,6 @@ __device__ __forceinline__ int row_exponent(unsigned top) { return top == 0 ? 0 
 __device__ __forceinline__ float e4m3_value(unsigned byte) {
   return __half2float(__half(__nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)byte, __NV_E4M3)));
 }
-
 __device__ __forceinline__ float reciprocal(float v) {        // off by 2^-22 of itself at most
   float r;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
@@ -143,16 +155,16 @@ __device__ __forceinline__ float reciprocal(float v) {        // off by 2^-22 of
 // are divided, and the quotient's rounding does not take them across t; a bfloat16 value (8 bits) and 6 t (7 bits) are equal or 2^-8 of
 // themselves apart, so that the product with 1 / 6, rounded to 12 bits, is t exactly where the quotient is and on its side of t elsewhere.
 template <typename T, int FORMAT>
-__device__ __forceinline__ unsigned scale_byte(unsigned top, int row_e) {
+__device__ __forceinline__ unsigned scale_byte(unsigned top, float row_up) {
   if (FORMAT == MXFP4) return top == 0 ? 0u : (unsigned)max((int)(top >> 23) - 2, 0);       // 253 at most
-  float wanted = __uint_as_float(top) * power_of_two(-row_e);
+  float wanted = __uint_as_float(top) * row_up;
   if (sizeof(T) == 4) wanted = __fdiv_rn(wanted, 6.f);
   else wanted = __uint_as_float((__float_as_uint(wanted * (1.f / 6.f)) + 0x800u) & 0xfffff000u);
   const unsigned byte = __nv_cvt_float_to_fp8(wanted, __NV_SATFINITE, __NV_E4M3);
   return top == 0 ? 0u : max(byte, 1u);
 }
 
-// A unit's codes.
+// A unit's codes.  row_up: 1 / row scale.
 //
 // nvfp4: value / row scale is exact.  The quotient by the block's scale s may be rounded before it is rounded to a code, but not across a
 // halfway point t.  32-bit values: the division's own rounding keeps the two apart (value and s t are 32-bit numbers, so they
@@ -160,28 +172,30 @@ __device__ __forceinline__ unsigned scale_byte(unsigned top, int row_e) {
 // themselves, 2^-10 or more in the quotient: value * (1 / s), which is off by 2^-21 of itself, is rounded to a multiple of 2^-13 (added to
 // 1536, whose steps these are, and taken away again), which makes it t exactly where the quotient is and leaves it on its side of t elsewhere.
 template <typename T, int FORMAT>
-__device__ __forceinline__ unsigned unit_codes(const Unit<T> &x, unsigned byte, int row_e) {
-  float v[UNIT];
-  x.values(v);
+__device__ __forceinline__ uint2 unit_codes(const Unit<T> &x, unsigned byte, float row_up) {
+  float2 v[UNIT / 2];
+#pragma unroll
+  for (int i = 0; i < UNIT / 2; ++i) v[i] = x.two(i);
   if (FORMAT == MXFP4) {
     const float up = power_of_two(127 - (int)byte);
 #pragma unroll
-    for (int i = 0; i < UNIT; ++i) v[i] *= up;
+    for (int i = 0; i < UNIT / 2; ++i) v[i] = mul_two(v[i], make_float2(up, up));
   } else if (sizeof(T) == 4) {
-    const float up = power_of_two(-row_e), s = byte == 0 ? 1.f : e4m3_value(byte);       // an empty block is zeros by any scale
+    const float s = byte == 0 ? 1.f : e4m3_value(byte);                // an empty block is zeros by any scale
 #pragma unroll
-    for (int i = 0; i < UNIT; ++i) v[i] = __fdiv_rn(v[i] * up, s);
+    for (int i = 0; i < UNIT / 2; ++i) v[i] = make_float2(__fdiv_rn(v[i].x * row_up, s), __fdiv_rn(v[i].y * row_up, s));
   } else {
-    if (row_e < -117) {                        // 1 / (row scale * s) would be beyond 32 bits: the row in two steps
+    if (row_up > 1.7e35f) {                    // 2^117: 1 / (row scale * s) would be beyond 32 bits, the row in two steps
+      const float up = power_of_two(64);
 #pragma unroll
-      for (int i = 0; i < UNIT; ++i) v[i] *= power_of_two(64);
-      row_e += 64;
+      for (int i = 0; i < UNIT / 2; ++i) v[i] = mul_two(v[i], make_float2(up, up));
+      row_up *= power_of_two(-64);
     }
-    const float by = byte == 0 ? 0.f : reciprocal(e4m3_value(byte)) * power_of_two(-row_e);
+    const float by = byte == 0 ? 0.f : reciprocal(e4m3_value(byte)) * row_up;
 #pragma unroll
-    for (int i = 0; i < UNIT; ++i) v[i] = __fmaf_rn(v[i], by, 1536.f) - 1536.f;
+    for (int i = 0; i < UNIT / 2; ++i) v[i] = add_two(fma_two(v[i], make_float2(by, by), make_float2(1536.f, 1536.f)), make_float2(-1536.f, -1536.f));
   }
-  return pack_codes(v);
+  return make_uint2(pack_codes(v), pack_codes(v + 4));
 }
 
 struct Fp4Out {
@@ -191,20 +205,15 @@ struct Fp4Out {
   long long sf_tiles;           // scale tiles of 128 rows along K
 };
 
-// The block's maximum from its lanes' (all lanes of the warp take part).
-template <int FORMAT>
-__device__ __forceinline__ unsigned block_top(unsigned top) {
-  top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-  return FORMAT == MXFP4 ? max(top, __shfl_xor_sync(0xffffffffu, top, 2)) : top;
-}
-// A unit into its codes, with its block's scale byte; a lane in 8 (nvfp4) or 16 (mxfp4) stores the scales of four blocks.  All lanes take part;
-// the warp's 32 units are 256 of K within the row (`there`), or none is.
+// A unit into its codes, with its block's scale byte; a lane in 4 (nvfp4) or 8 (mxfp4) stores the scales of four blocks.  All lanes take part;
+// the units of 256 of K lie within the row (`there`), or none does.
 template <typename T, int FORMAT>
-__device__ __forceinline__ void put_unit(const Fp4Out &o, long long row, int u, bool there, const Unit<T> &x, unsigned top, int row_e) {
-  const unsigned byte = scale_byte<T, FORMAT>(block_top<FORMAT>(top), row_e);
-  const unsigned codes = unit_codes<T, FORMAT>(x, byte, row_e);
-  if (there && u * 4 < o.ldc) *reinterpret_cast<unsigned *>(o.codes + row * o.ldc + u * 4) = codes;
-  constexpr int LANES = FORMAT == NVFP4 ? 2 : 4, PER = 4 * LANES;     // lanes to a block, to four
+__device__ __forceinline__ void put_unit(const Fp4Out &o, long long row, int u, bool there, const Unit<T> &x, unsigned top, float row_up) {
+  if (FORMAT == MXFP4) top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+  const unsigned byte = scale_byte<T, FORMAT>(top, row_up);
+  const uint2 codes = unit_codes<T, FORMAT>(x, byte, row_up);
+  if (there && u * 8 < o.ldc) *reinterpret_cast<uint2 *>(o.codes + row * o.ldc + u * 8) = codes;
+  constexpr int LANES = FORMAT == NVFP4 ? 1 : 2, PER = 4 * LANES;     // lanes to a block, to four
   unsigned w = byte | __shfl_xor_sync(0xffffffffu, byte, LANES) << 8;
   w |= __shfl_xor_sync(0xffffffffu, w, 2 * LANES) << 16;
   if (there && u % PER == 0)
@@ -214,19 +223,20 @@ __device__ __forceinline__ float row_scale_of(int format, unsigned top) {
   return top >= 0x7f800000u ? __uint_as_float(0x7fffffffu) : power_of_two(format == NVFP4 ? row_exponent(top) : 0);
 }
 
-// Short rows: a warp to ROWS rows at once, HELD units of each in a lane's registers between the row's maximum and the codes.
-template <typename T, int FORMAT, int ROWS, int HELD>
+// Short rows: LANES lanes to a row, ROWS rows of each such group at once, HELD units of each in a lane's registers between the row's maximum and
+// the codes.
+template <typename T, int FORMAT, int LANES, int ROWS, int HELD>
 __global__ void __launch_bounds__(128)
 fp4_quantize_warp_kernel(const T *x, long long ldx, Fp4Out o, long long rows, int K, int n_units, int vec) {
   grid_dependents_launch();
   grid_dependency_wait();
-  const int lane = threadIdx.x & 31;
-  const long long row0 = ((long long)blockIdx.x * 4 + threadIdx.x / 32) * ROWS;
+  const int lane = threadIdx.x % LANES;
+  const long long row0 = ((long long)blockIdx.x * (128 / LANES) + threadIdx.x / LANES) * ROWS;
   Unit<T> held[ROWS][HELD];
 #pragma unroll
   for (int r = 0; r < ROWS; ++r)
 #pragma unroll
-    for (int i = 0; i < HELD; ++i) held[r][i] = fetch_unit(x + (row0 + r) * ldx, lane + i * 32, row0 + r < rows ? K : 0, vec);
+    for (int i = 0; i < HELD; ++i) held[r][i] = fetch_unit(x + (row0 + r) * ldx, lane + i * LANES, row0 + r < rows ? K : 0, vec);
 #pragma unroll
   for (int r = 0; r < ROWS; ++r) {
     unsigned tu[HELD], top = 0;
@@ -235,12 +245,17 @@ fp4_quantize_warp_kernel(const T *x, long long ldx, Fp4Out o, long long rows, in
       tu[i] = held[r][i].top();
       top = max(top, tu[i]);
     }
-    top = __reduce_max_sync(0xffffffffu, top);
+    if (LANES == 32) {
+      top = __reduce_max_sync(0xffffffffu, top);
+    } else {
+#pragma unroll
+      for (int d = LANES / 2; d > 0; d /= 2) top = max(top, __shfl_xor_sync(0xffffffffu, top, d));
+    }
     const bool there = row0 + r < rows;
     if (lane == 0 && there) o.row_scale[row0 + r] = row_scale_of(FORMAT, top);
+    const float row_up = power_of_two(-row_exponent(top));
 #pragma unroll
-    for (int i = 0; i < HELD; ++i)
-      put_unit<T, FORMAT>(o, row0 + r, lane + i * 32, there && lane + i * 32 < n_units, held[r][i], tu[i], row_exponent(top));
+    for (int i = 0; i < HELD; ++i) put_unit<T, FORMAT>(o, row0 + r, lane + i * LANES, there && lane + i * LANES < n_units, held[r][i], tu[i], row_up);
   }
 }
 
@@ -274,15 +289,15 @@ fp4_quantize_block_kernel(const T *x, long long ldx, Fp4Out o, long long rows, i
 #pragma unroll
   for (int w = 0; w < THREADS / 32; ++w) top = max(top, tops[w]);
   if (t == 0) o.row_scale[row] = row_scale_of(FORMAT, top);
-  const int row_e = row_exponent(top);
+  const float row_up = power_of_two(-row_exponent(top));
   if (HELD) {
 #pragma unroll
-    for (int i = 0; i < HELD; ++i) put_unit<T, FORMAT>(o, row, t + i * THREADS, t + i * THREADS < n_units, held[i], tu[i], row_e);
+    for (int i = 0; i < HELD; ++i) put_unit<T, FORMAT>(o, row, t + i * THREADS, t + i * THREADS < n_units, held[i], tu[i], row_up);
   } else {
 #pragma unroll 2
-    for (int u = t; u < n_units; u += THREADS) {            // n_units is a multiple of 32: a warp is in or out
+    for (int u = t; u < (n_units + 31) / 32 * 32; u += THREADS) {      // whole warps
       const Unit<T> v = fetch_unit(r, u, K, vec);
-      put_unit<T, FORMAT>(o, row, u, true, v, v.top(), row_e);
+      put_unit<T, FORMAT>(o, row, u, u < n_units, v, v.top(), row_up);
     }
   }
 }
@@ -298,17 +313,18 @@ int launch_quantize(const void *x, long long ldx, const Fp4Out &o, long long row
                    "fp4_quantize launch");                                                                                               \
     return LLM_OK;                                                                                                                        \
   } while (0)
-#define FP4_WARP(ROWS, HELD) FP4_GO((fp4_quantize_warp_kernel<T, FORMAT, ROWS, HELD>), (rows + 4 * ROWS - 1) / (4 * ROWS), 128)
+#define FP4_WARP(LANES, ROWS, HELD) \
+  FP4_GO((fp4_quantize_warp_kernel<T, FORMAT, LANES, ROWS, HELD>), (rows + 128 / LANES * ROWS - 1) / (128 / LANES * ROWS), 128)
 #define FP4_BLOCK(THREADS, HELD) FP4_GO((fp4_quantize_block_kernel<T, FORMAT, THREADS, HELD>), rows, THREADS)
-  if (n_units <= 32) FP4_WARP(4, 1);
-  if (n_units <= 64) FP4_WARP(2, 2);
-  if (n_units <= 256 && rows <= 4 * sm_count()) FP4_BLOCK(256, 1);
-  if (n_units <= 128) FP4_WARP(1, 4);
-  if (n_units <= 256) FP4_WARP(1, 8);
+  if (n_units <= 16) FP4_WARP(16, 2, 1);
+  if (n_units <= 32) FP4_WARP(32, 2, 1);
+  if (n_units <= 128 && rows <= 4 * sm_count()) FP4_BLOCK(128, 1);
+  if (n_units <= 64) FP4_WARP(32, 1, 2);
+  if (n_units <= 128) FP4_WARP(32, 1, 4);
+  if (n_units <= 256) FP4_BLOCK(128, 2);
   if (n_units <= 512) FP4_BLOCK(256, 2);
-  if (n_units <= 1024) FP4_BLOCK(256, 4);
-  if (n_units <= 2048) FP4_BLOCK(512, 4);
-  if (n_units <= 4096) FP4_BLOCK(1024, 4);
+  if (n_units <= 1024) FP4_BLOCK(512, 2);
+  if (n_units <= 2048) FP4_BLOCK(1024, 2);
   FP4_BLOCK(1024, 0);
 #undef FP4_WARP
 #undef FP4_BLOCK
@@ -316,17 +332,18 @@ int launch_quantize(const void *x, long long ldx, const Fp4Out &o, long long row
 }
 
 // ---------------------------------------------------------------- back
+constexpr int EIGHT = 8;                       // values that a lane brings back at once: 16 bytes of bfloat16
 __device__ __forceinline__ float scale_value(int format, unsigned byte) {
   if (format == NVFP4) return e4m3_value(byte & 0x7f);
   return byte == 0 ? __uint_as_float(0x00400000u) : byte == 255 ? __uint_as_float(0x7fffffffu) : __uint_as_float(byte << 23);
 }
-__device__ __forceinline__ void store_unit(__nv_bfloat16 *p, const float (&v)[UNIT]) {
+__device__ __forceinline__ void store_unit(__nv_bfloat16 *p, const float (&v)[EIGHT]) {
   __nv_bfloat162 h[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) h[i] = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
   *reinterpret_cast<uint4 *>(p) = *reinterpret_cast<const uint4 *>(h);
 }
-__device__ __forceinline__ void store_unit(float *p, const float (&v)[UNIT]) {
+__device__ __forceinline__ void store_unit(float *p, const float (&v)[EIGHT]) {
   reinterpret_cast<float4 *>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
   reinterpret_cast<float4 *>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
 }
@@ -355,8 +372,8 @@ fp4_dequantize_kernel(const unsigned char *codes, const unsigned char *scales, c
 #pragma unroll
       for (int i = 0; i < PER; ++i) {
         const int u = u0 + i * 32, block = u / LANES;
-        c[r * PER + i] = u * UNIT < end ? *reinterpret_cast<const unsigned *>(codes + row * ldc + u * 4) : 0;
-        byte[r * PER + i] = u * UNIT < end ? sf[(block / 4) * SF_TILE + block % 4] : 0;
+        c[r * PER + i] = u * EIGHT < end ? *reinterpret_cast<const unsigned *>(codes + row * ldc + u * 4) : 0;
+        byte[r * PER + i] = u * EIGHT < end ? sf[(block / 4) * SF_TILE + block % 4] : 0;
       }
     }
 #pragma unroll
@@ -366,22 +383,22 @@ fp4_dequantize_kernel(const unsigned char *codes, const unsigned char *scales, c
 #pragma unroll
       for (int i = 0; i < PER; ++i) {
         const int u = u0 + i * 32;
-        if (u * UNIT >= K) break;
-        const float s = scale_value(FORMAT, byte[r * PER + i]);
-        float v[UNIT];
+        if (u * EIGHT >= K) break;
+        const float by = scale_value(FORMAT, byte[r * PER + i]) * rs[r];       // exact: a scale has four bits
+        float v[EIGHT];
 #pragma unroll
-        for (int j = 0; j < UNIT / 2; ++j) {
+        for (int j = 0; j < EIGHT / 2; ++j) {
           const float2 f = __half22float2(__half2(__nv_cvt_fp4x2_to_halfraw2((__nv_fp4x2_storage_t)(c[r * PER + i] >> 8 * j & 0xff), __NV_E2M1)));
-          v[2 * j] = f.x * s * rs[r];
-          v[2 * j + 1] = f.y * s * rs[r];
+          v[2 * j] = f.x * by;
+          v[2 * j + 1] = f.y * by;
         }
-        TO *p = out + row * ldo + u * UNIT;
-        if (vec && (u + 1) * UNIT <= K) {
+        TO *p = out + row * ldo + u * EIGHT;
+        if (vec && (u + 1) * EIGHT <= K) {
           store_unit(p, v);
         } else {
 #pragma unroll
-          for (int j = 0; j < UNIT; ++j)
-            if (u * UNIT + j < K) p[j] = from_float<TO>(v[j]);
+          for (int j = 0; j < EIGHT; ++j)
+            if (u * EIGHT + j < K) p[j] = from_float<TO>(v[j]);
         }
       }
     }
@@ -390,7 +407,7 @@ fp4_dequantize_kernel(const unsigned char *codes, const unsigned char *scales, c
 
 template <typename TO, int FORMAT, int PER>
 int launch_dequantize(const Fp4DequantizeCall &c) {
-  const long long K = c.cols, pieces = PER < 4 ? 1 : (K + 128 * UNIT - 1) / (128 * UNIT), jobs = (c.rows + 4 / PER - 1) / (4 / PER) * pieces;
+  const long long K = c.cols, pieces = PER < 4 ? 1 : (K + 128 * EIGHT - 1) / (128 * EIGHT), jobs = (c.rows + 4 / PER - 1) / (4 / PER) * pieces;
   const long long blocks = (jobs + 7) / 8, most = 8ll * 4 * sm_count();
   const int vec = (uintptr_t)c.out % 16 == 0 && c.ldo * (long long)sizeof(TO) % 16 == 0;
   LLM_CHECK_CUDA(llm_launch(fp4_dequantize_kernel<TO, FORMAT, PER>, dim3((unsigned)(blocks < most ? blocks : most)), dim3(256), 0, (cudaStream_t)c.stream,
@@ -401,8 +418,8 @@ int launch_dequantize(const Fp4DequantizeCall &c) {
 }
 template <typename TO, int FORMAT>
 int dispatch_dequantize(const Fp4DequantizeCall &c) {
-  if (c.cols <= 32 * UNIT) return launch_dequantize<TO, FORMAT, 1>(c);
-  if (c.cols <= 64 * UNIT) return launch_dequantize<TO, FORMAT, 2>(c);
+  if (c.cols <= 32 * EIGHT) return launch_dequantize<TO, FORMAT, 1>(c);
+  if (c.cols <= 64 * EIGHT) return launch_dequantize<TO, FORMAT, 2>(c);
   return launch_dequantize<TO, FORMAT, 4>(c);
 }
 
