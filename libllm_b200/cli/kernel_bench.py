@@ -5,6 +5,8 @@
     python -m libllm_b200.cli.kernel_bench attention_prefill --tokens 2048
     python -m libllm_b200.cli.kernel_bench layer_products --m 8      # the four products of one layer
     python -m libllm_b200.cli.kernel_bench chain_layer --m 8         # a layer's products and norms as one launch
+    python -m libllm_b200.cli.kernel_bench fp4 --m 8 --n 128256 --k 2048 --format nvfp4    # into four bits, back, the product
+    python -m libllm_b200.cli.kernel_bench adjust --batch 64 --context 2048                # penalties, bias and mask on logits
 
 One JSON line per run: microseconds per launch (CUDA events on the launching stream,
 after warm-up, with a buffer larger than L2 written between launches), the bytes the
@@ -324,7 +326,40 @@ def bench_gemm(args, timer):
     report("library_gemm", us, flops=2 * M * N * K, bytes_moved=2 * (M * K + N * K + M * N), m=M, n=N, k=K)
 
 
-KERNELS = {"gemv": bench_gemv, "layer_products": bench_layer_products, "attention_decode": bench_attention_decode,
+def bench_fp4(args, timer):
+    """A matrix [n, k] into four bits and back, and the product of m tokens with it (both held in four bits)."""
+    import torch
+    from ..csrc import ops
+    M, N, K, f = args.m, args.n, args.k, args.format
+    w = (torch.randn(N, K, device="cuda") * 0.02).to(torch.bfloat16)
+    qw, qx = ops.fp4_quantize(w, f), ops.fp4_quantize(torch.randn(M, K, device="cuda").to(torch.bfloat16), f)
+    back, out = torch.empty_like(w), torch.empty(M, N, dtype=torch.bfloat16 if M > 64 else torch.float32, device="cuda")
+    us = timer.run(lambda: ops.fp4_quantize(w, f, out=qw))
+    report("fp4_quantize", us, bytes_moved=2 * N * K + qw.nbytes, n=N, k=K, format=f)
+    us = timer.run(lambda: ops.fp4_dequantize(qw, out=back))
+    report("fp4_dequantize", us, bytes_moved=2 * N * K + qw.nbytes, n=N, k=K, format=f)
+    us = timer.run(lambda: ops.fp4_gemm(qx, qw, out=out))
+    report("fp4_gemm", us, bytes_moved=qw.nbytes + qx.nbytes + out.numel() * out.element_size(), flops=2 * M * N * K, m=M, n=N, k=K, format=f)
+    ops.check_tc_status()
+
+
+def bench_adjust(args, timer):
+    """Penalties for histories of --context tokens, a bias and a mask on --batch rows of --vocab logits; then each alone."""
+    import torch
+    from ..csrc import ops
+    B, V, L = args.batch, args.vocab, args.context
+    logits, out = torch.randn(B, V, device="cuda"), torch.empty(B, V, device="cuda")
+    history = dict(history=(V * torch.rand(B, L, device="cuda") ** 4).int().clamp_(max=V - 1), repetition=1.2, presence=0.3, frequency=0.1,
+                   lengths=torch.full((B,), L, dtype=torch.int32, device="cuda"))
+    bias = dict(bias=torch.randn(V, device="cuda"))
+    allowed = dict(allowed=torch.randint(-2 ** 31, 2 ** 31, (B, (V + 31) // 32), device="cuda", dtype=torch.int64).int())
+    for name, kw, extra in (("all", {**history, **bias, **allowed}, 4 * B * L + 4 * V + B * V // 8), ("history", history, 4 * B * L),
+                            ("bias", bias, 4 * V), ("mask", allowed, B * V // 8)):
+        us = timer.run(lambda: ops.adjust_logits(logits, out=out, **kw))
+        report(f"adjust_logits ({name})", us, bytes_moved=8 * B * V + extra, batch=B, vocab=V, history=L)
+
+
+KERNELS = {"fp4": bench_fp4, "adjust": bench_adjust, "gemv": bench_gemv, "layer_products": bench_layer_products, "attention_decode": bench_attention_decode,
            "attention_prefill": bench_attention_prefill, "add_rmsnorm": bench_add_rmsnorm,
            "sampling": bench_sampling, "gemm": bench_gemm, "chain_layer": bench_chain_layer}
 
@@ -356,6 +391,7 @@ def main(argv=None) -> int:
     ap.add_argument("--generic", action="store_true", help="attention_prefill: time the general kernel")
     ap.add_argument("--iters", type=int, default=20)
     ap.add_argument("--warmup", type=int, default=3)
+    ap.add_argument("--format", choices=["nvfp4", "mxfp4"], default="nvfp4", help="fp4: the format")
     ap.add_argument("--no-flush", action="store_true", help="do not write a buffer larger than L2 between launches")
     args = ap.parse_args(argv)
     import torch

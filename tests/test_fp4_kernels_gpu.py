@@ -273,3 +273,54 @@ def test_products_behind_products_read_what_the_last_one_left():
         for _ in range(4):
             fast = o.fp4_gemm(o.fp4_quantize(fast, format), o.fp4_quantize(w, format), out_dtype=torch.bfloat16)
         assert torch.equal(fast, y)
+
+
+def test_two_streams_at_once():
+    """Products, parts of K among them, and their rows on two streams: nothing is shared between calls."""
+    o = ops()
+    sizes = [(5, 2048, 4096), (300, 700, 512), (20, 1000, 8192), (100, 600, 1024)]
+    xs = [rows_like(M, K, i).to(DEV) for i, (M, _, K) in enumerate(sizes)]
+    ws = [o.fp4_quantize(rows_like(N, K, 10 + i, spread=2).to(DEV)) for i, (_, N, K) in enumerate(sizes)]
+    want = [o.fp4_gemm(o.fp4_quantize(x), w) for x, w in zip(xs, ws)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [[], []]
+    for _ in range(20):
+        for k, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                for x, w in zip(xs[k::2], ws[k::2]):
+                    got[k].append(o.fp4_gemm(o.fp4_quantize(x), w))
+    torch.cuda.synchronize()
+    for k in range(2):
+        for i, y in enumerate(got[k]):
+            assert torch.equal(y, want[k + 2 * (i % 2)])
+    o.check_tc_status()
+
+
+def test_offsets_beyond_32_bits():
+    """Rows that lie 2^31 elements and more apart, in and out."""
+    o = ops()
+    far = 2 ** 31 + 2 ** 27
+    x, w = rows_like(2, 500, 1), rows_like(300, 500, 2)
+    room = torch.zeros(far + 1024, dtype=torch.bfloat16, device=DEV)
+    rows = room.as_strided((2, 500), (far, 1))
+    rows.copy_(x)
+    q, qw = o.fp4_quantize(rows), o.fp4_quantize(w.to(DEV))
+    same_values(x, "nvfp4", o.fp4_dequantize(q))
+    rows.zero_()
+    o.fp4_dequantize(q, out=rows)
+    same_values(x, "nvfp4", rows)
+    want = o.fp4_gemm(q, qw, out_dtype=torch.bfloat16)
+    out = room.as_strided((2, 300), (far, 1))
+    o.fp4_gemm(q, qw, out=out)
+    assert torch.equal(out, want)
+    # a prompt's rows: the last of 300 lies more than 2^31 elements from the first
+    step = far // 299 // 8 * 8
+    x = rows_like(300, 500, 3).to(DEV)
+    q = o.fp4_quantize(x)
+    want = o.fp4_gemm(q, qw, out_dtype=torch.bfloat16)
+    for at in (0, 3):
+        room.zero_()
+        out = room[at:].as_strided((300, 300), (step - 4, 1)) if at else room.as_strided((300, 300), (step, 1))
+        o.fp4_gemm(q, qw, out=out)
+        assert torch.equal(out, want) and int((room != 0).sum()) == int((want != 0).sum())

@@ -183,3 +183,25 @@ def test_captured_and_replayed_with_longer_histories():
         graph.replay()
     s.synchronize()
     assert torch.equal(out, o.adjust_logits(x, **kw))
+
+
+def test_offsets_beyond_32_bits():
+    o = ops()
+    g = torch.Generator().manual_seed(7)
+    B, V, L, far = 2, 1000, 300, 2 ** 31 + 12
+    room, ints = torch.zeros(far + 2048, device=DEV), torch.zeros(far + 2048, dtype=torch.int32, device=DEV)
+    logits, history = torch.randn(B, V, generator=g).to(DEV), history_of(B, L, V, g).to(DEV)
+    lengths = torch.full((B,), L, dtype=torch.int32, device=DEV)
+    bias, allowed = torch.randn(B, V, generator=g).to(DEV), words_of((B,), V, g).to(DEV)
+    want = o.adjust_logits(logits, history=history, lengths=lengths, repetition=1.5, frequency=0.25, bias=bias, allowed=allowed)
+    x, h = room.as_strided((B, V), (far, 1)), ints.as_strided((B, L), (far, 1))
+    x.copy_(logits)
+    h.copy_(history)
+    kw = dict(history=h, lengths=lengths, repetition=1.5, frequency=0.25, allowed=allowed)
+    assert torch.equal(o.adjust_logits(x, bias=bias, **kw), want)
+    o.adjust_logits(x, out=x, bias=bias, **kw)
+    assert torch.equal(x, want) and int((room != 0).sum()) == int((want != 0).sum())
+    b, a = room.as_strided((B, V), (far, 1)), ints.as_strided((B, allowed.shape[1]), (far, 1))
+    b.copy_(bias)
+    a.copy_(allowed)
+    assert torch.equal(o.adjust_logits(logits, bias=b, history=history, lengths=lengths, repetition=1.5, frequency=0.25, allowed=a), want)
