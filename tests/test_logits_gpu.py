@@ -46,8 +46,9 @@ def plain(logits, history=None, slots=None, lengths=None, repetition=1.0, presen
 
 
 def check(logits, **kw):
-    """A logit goes through at most five roundings of 32 bits: a division, a product and two sums, of values no larger than the largest that
-    occurs on the way (the logit times its repetition, the penalty, the bias), and the plain form's narrowing to what is compared."""
+    """A logit goes through six roundings of 32 bits: two for the division by its repetition, two for the penalty, one each for taking that away and adding
+    the bias.  The first two are of the logit's size, the next two of the penalty's, the last of all together: five half steps of the sum of
+    what occurs on the way (the logit times its repetition, the penalty, the bias) hold them, and the plain form's narrowing."""
     o = ops()
     dev = {k: v.to(DEV) if isinstance(v, torch.Tensor) else v for k, v in kw.items()}
     keep = logits.to(DEV)
@@ -128,6 +129,19 @@ def test_infinities_and_nan():
     got = check(row[None], repetition=1.0, allowed=allowed, **kw)
     assert got[0, 0] == -INF and got[0, 2] == -INF, "a masked place is minus infinity whatever stands there"
     check(row[None], bias=torch.full((8,), -INF))
+
+
+@pytest.mark.parametrize("repetition", [2.0 ** -140, 1e-39, 2.0 ** -126, 3e-38, 2.0 ** 126, 3e38, 1.0 + 2.0 ** -23, 1.0 - 2.0 ** -24])
+def test_penalties_whose_reciprocal_is_no_ordinary_number(repetition):
+    row = torch.tensor([1e-40, -1e-40, 2.0 ** -149, 1e-38, -1e-38, 1.0, -1.0, 3e38, -3e38, 0.0, 5e-20, -7e20])
+    history = torch.arange(12).int()[None]
+    got = ops().adjust_logits(row[None].to(DEV), history=history.to(DEV), lengths=torch.tensor([12], dtype=torch.int32, device=DEV),
+                              repetition=torch.tensor([repetition], device=DEV))[0].cpu()
+    rep = torch.tensor(repetition).double()                     # as 32 bits hold it
+    want = torch.where(row > 0, row.double() / rep, row.double() * rep)
+    tol = want.abs() * 2.0 ** -22 + 2.0 ** -149
+    held = want.float().double()                                # infinite where 32 bits do not reach
+    assert ((got.double() == held) | ((got.double() - want).abs() <= tol)).all(), (got, want)
 
 
 def test_a_row_that_allows_nothing_is_still_sampled():
