@@ -5,7 +5,6 @@ a tensor that is not on a CUDA device is an error."""
 from __future__ import annotations
 
 import ctypes
-import math
 import struct
 from ctypes import c_char_p, c_float, c_int, c_longlong, c_void_p
 from typing import Optional
@@ -402,16 +401,19 @@ def _other_device(t: torch.Tensor) -> None:
     raise InvalidArgError(f"a tensor lies on '{t.device}', the launch goes to the current device 'cuda:{torch.cuda.current_device()}'")
 
 
+_F32_MOST, _F32_LEAST = (2 - 2.0 ** -23) * 2.0 ** 127, 2.0 ** -149
+
+
 def _per_row(name: str, v, rows: int, *, positive: bool = False):
-    """A number for all rows, or a 32-bit tensor with one per row: (the tensor or None, its address or 0, the number)."""
+    """A number for all rows, or a 32-bit tensor with one per row: (the tensor or None, its address or 0, the number, which 32 bits hold)."""
     if type(v) is not float:
         if isinstance(v, torch.Tensor):
             if v.dtype != _F32 or v.dim() != 1 or v.size(0) != rows or not v.is_contiguous():
                 raise InvalidArgError(f"adjust_logits: {name} is a number or a contiguous float32 tensor with one per row ({rows})")
             return v, v.data_ptr(), 0.0
         v = float(v)
-    if not math.isfinite(v) or (positive and v <= 0):
-        raise InvalidArgError(f"adjust_logits: {name} must be a finite{' positive' if positive else ''} number, got {v}")
+    if not abs(v) <= _F32_MOST or (positive and v < _F32_LEAST):
+        raise InvalidArgError(f"adjust_logits: {name} must be a finite{' positive' if positive else ''} number of 32 bits, got {v}")
     return None, 0, v
 
 
@@ -530,6 +532,15 @@ class Fp4Matrix:
         q.data = data
         return q
 
+    def check(self) -> None:
+        """The memory is still what rows, cols and format need (all of them can be set)."""
+        d = self.data
+        if self._layout is not _fp4_layouts.get((self.rows, self.cols, self.format)):
+            self._layout = _fp4_layout(self.rows, self.cols, self.format)
+        if d.dtype != torch.uint8 or d.dim() != 1 or not d.is_contiguous() or d.size(0) != self._layout[4]:
+            raise InvalidArgError(f"fp4: {self.format} [{self.rows}, {self.cols}] lies in {self._layout[4]} contiguous bytes, data is "
+                                  f"{str(d.dtype).replace('torch.', '')} {list(d.shape)}")
+
     @property
     def device(self):
         return self.data.device
@@ -595,6 +606,7 @@ def fp4_quantize(x: torch.Tensor, format: str = "nvfp4", out: Optional[Fp4Matrix
     else:
         if out.rows != rows or out.cols != cols or out.format != format:
             raise InvalidArgError(f"fp4_quantize: out is {out.format} [{out.rows}, {out.cols}], x becomes {format} [{rows}, {cols}]")
+        out.check()
         stream = _same_device(x, out.data)
     number, _, scales, row, _ = out._layout
     p = out.data.data_ptr()
@@ -611,6 +623,7 @@ def fp4_dequantize(q: Fp4Matrix, dtype: torch.dtype = torch.float32, out: Option
         if values is not None:
             _launched("fp4", "fp4_dequantize", values)
             return values
+    q.check()
     if out is None:
         ldo = cols
         stream = _same_device(q.data)
@@ -643,6 +656,8 @@ def fp4_gemm(x: Fp4Matrix, w: Fp4Matrix, out: Optional[torch.Tensor] = None, out
         if result is not None:
             _launched("fp4", "fp4_gemm", result)
             return result
+        x.check()
+        w.check()
         stream = _same_device(wd, xd)
         ldo = N
         out = torch.empty(M, N, dtype=out_dtype, device=wd.device)
@@ -650,6 +665,8 @@ def fp4_gemm(x: Fp4Matrix, w: Fp4Matrix, out: Optional[torch.Tensor] = None, out
         dt = dtype_code(out.dtype)
         if out.shape != (M, N) or (N > 1 and out.stride(1) != 1) or (M > 1 and out.stride(0) < N):
             raise InvalidArgError(f"fp4_gemm: out is [{M}, {N}] with neighbouring columns and rows of its own")
+        x.check()
+        w.check()
         stream = _same_device(wd, xd, out)
         ldo = out.stride(0)
     number, _, xs, xr, _ = x._layout

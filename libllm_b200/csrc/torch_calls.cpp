@@ -181,7 +181,7 @@ bool per_row(const at::Tensor &t, at::ScalarType type, long long rows) {
 void penalty(PyObject *o, long long rows, const Place &place, bool positive, const float **p, double *all) {
   if (PyFloat_CheckExact(o)) {
     *all = PyFloat_AS_DOUBLE(o);
-    need(std::isfinite(*all) && (!positive || *all > 0));
+    need(std::isfinite((float)*all) && (!positive || (float)*all > 0));
     return;
   }
   const at::Tensor &t = tensor(o);

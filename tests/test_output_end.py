@@ -96,3 +96,30 @@ def test_logits_and_what_goes_with_them(kw):
     logits = kw.pop("logits", torch.zeros(B, V))
     with pytest.raises(InvalidArgError):
         ops.adjust_logits(logits, **kw)
+
+
+@pytest.mark.parametrize("kw", [dict(repetition=1e39), dict(repetition=1e-46), dict(repetition=10 ** 39), dict(presence=-1e39), dict(frequency=1e300)])
+def test_penalties_that_32_bits_do_not_hold(kw):
+    with pytest.raises(InvalidArgError):
+        ops.adjust_logits(torch.zeros(B, V), **kw)
+
+
+def changed(**kw):
+    q = matrix(4, 64)
+    for name, v in kw.items():
+        setattr(q, name, v)
+    return q
+
+
+@pytest.mark.parametrize("kw", [dict(data=matrix(4, 64).data[:-1]), dict(data=torch.zeros(2 * matrix(4, 64).nbytes, dtype=torch.uint8)[::2]),
+                                dict(data=torch.zeros(matrix(4, 64).nbytes, dtype=torch.int8)), dict(rows=400), dict(cols=6400), dict(cols=0)])
+def test_matrices_whose_memory_is_not_theirs(kw):
+    rows, cols = kw.get("rows", 4), kw.get("cols", 64)
+    calls = [lambda q: ops.fp4_dequantize(q), lambda q: ops.fp4_dequantize(q, out=torch.zeros(rows, cols)),
+             lambda q: ops.fp4_gemm(q, ops.Fp4Matrix(3, max(cols, 1), "nvfp4", "cpu")),
+             lambda q: ops.fp4_gemm(q, ops.Fp4Matrix(3, max(cols, 1), "nvfp4", "cpu"), out=torch.zeros(rows, 3)),
+             lambda q: ops.fp4_gemm(ops.Fp4Matrix(3, max(cols, 1), "nvfp4", "cpu"), q),
+             lambda q: ops.fp4_quantize(torch.zeros(rows, max(cols, 1)), out=q)]
+    for call in calls:
+        with pytest.raises(InvalidArgError):
+            call(changed(**kw))
