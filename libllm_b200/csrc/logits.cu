@@ -63,10 +63,14 @@ __device__ __forceinline__ void count(unsigned *counts, int id, int v0, int n) {
   }
 }
 
-// AT threads to a slice.
+// AT threads to a slice.  Its logits are on their way while its history is counted: into shared memory where there are 256 threads (held in registers, 39
+// for 32, they left six CTAs to an SM: 64 rows of 128,256 with everything 19.4 us for 16.6, with a mask alone 14.1 for 11.5, 5.9 TB/s, cold
+// caches), into registers where there are 1,024 and time is what a load takes (7 rows of 50,257 with 5,000 ids 4.5 us for 5.0).
 template <bool VEC, int AT>
-__global__ void __launch_bounds__(AT) adjust_kernel(Adjust a) {
-  extern __shared__ __align__(16) unsigned counts[];
+__global__ void __launch_bounds__(AT, AT == 1024 ? 2 : VEC ? 7 : 6) adjust_kernel(Adjust a) {
+  constexpr bool HELD = AT == 1024;
+  extern __shared__ __align__(16) unsigned counts[];                     // [slice] with a history; then [slice] logits if not HELD
+  float *ahead = reinterpret_cast<float *>(counts) + (a.history ? a.slice : 0);
   grid_dependents_launch();
   const long long b = blockIdx.y;
   const int v0 = blockIdx.x * a.slice, n = min(a.slice, a.V - v0);
@@ -76,27 +80,29 @@ __global__ void __launch_bounds__(AT) adjust_kernel(Adjust a) {
   const float *x = a.logits + b * a.ld + v0, *bias = a.bias ? a.bias + b * a.ld_bias + v0 : nullptr;
   const unsigned *allowed = a.allowed ? a.allowed + b * a.ld_allowed : nullptr;
   float *out = a.out + b * a.ldo + v0;
-  // The slice's logits are on their way while the history is counted.
   const int place = !a.history ? -1 : a.slots ? a.slots[b] : (int)b;
   const int said = a.history ? a.lengths[b] : 0;
   constexpr int AHEAD = MOST_SLICE / AT / 4;
-  float4 held[AHEAD];
+  const unsigned ahead_at = (unsigned)__cvta_generic_to_shared(ahead);
+  unsigned words[VEC ? AHEAD : 1];             // the mask's, in time: 12.6 -> 11.5 us for a mask alone
+  float4 held[HELD ? AHEAD : 1];
   if (VEC) {
 #pragma unroll
     for (int j = 0; j < AHEAD; ++j) {
       const int i = (threadIdx.x + j * AT) * 4;
-      if (i + 4 <= n) held[j] = *reinterpret_cast<const float4 *>(x + i);
+      if (HELD && i + 4 <= n) held[HELD ? j : 0] = *reinterpret_cast<const float4 *>(x + i);
+      if (!HELD && i + 4 <= n) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(ahead_at + i * 4), "l"(x + i) : "memory");
+      if (allowed && i < n) words[j] = allowed[(v0 + i) >> 5];
+    }
+  } else if (HELD) {
+    float *v = reinterpret_cast<float *>(held);
+#pragma unroll
+    for (int j = 0; j < 4 * AHEAD; ++j) {
+      const int i = threadIdx.x + j * AT;
+      if (i < n) v[HELD ? j : 0] = x[i];
     }
   } else {
-#pragma unroll
-    for (int j = 0; j < AHEAD; ++j) {
-      float *v = reinterpret_cast<float *>(&held[j]);
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int i = threadIdx.x + (4 * j + k) * AT;
-        if (i < n) v[k] = x[i];
-      }
-    }
+    for (int i = threadIdx.x; i < n; i += AT) asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(ahead_at + i * 4), "l"(x + i) : "memory");
   }
   const Penalty pen = a.history ? Penalty(a.repetition.at(b), a.presence.at(b), a.frequency.at(b)) : Penalty(1.f, 0.f, 0.f);
   if (a.history) {
@@ -132,12 +138,13 @@ __global__ void __launch_bounds__(AT) adjust_kernel(Adjust a) {
     if (allowed && !(allowed[(v0 + i) >> 5] >> ((v0 + i) & 31) & 1)) v = -INFINITY;
     return v;
   };
+  if (!HELD) asm volatile("cp.async.wait_all;" ::: "memory");            // a thread reads what it copied itself
   if (VEC) {                                   // slices are multiples of 32 tokens
 #pragma unroll
     for (int j = 0; j < AHEAD; ++j) {
       const int i = (threadIdx.x + j * AT) * 4;
       if (i + 4 > n) break;
-      float4 v = held[j];
+      float4 v = HELD ? held[HELD ? j : 0] : *reinterpret_cast<const float4 *>(ahead + i);
       if (a.history) {
         const uint4 c = *reinterpret_cast<const uint4 *>(counts + i);
         if (c.x | c.y | c.z | c.w) {
@@ -155,7 +162,7 @@ __global__ void __launch_bounds__(AT) adjust_kernel(Adjust a) {
         v.w += w.w;
       }
       if (allowed) {
-        const unsigned bits = allowed[(v0 + i) >> 5] >> ((v0 + i) & 31);
+        const unsigned bits = words[j] >> ((v0 + i) & 31);
         if (!(bits & 1)) v.x = -INFINITY;
         if (!(bits & 2)) v.y = -INFINITY;
         if (!(bits & 4)) v.z = -INFINITY;
@@ -165,15 +172,20 @@ __global__ void __launch_bounds__(AT) adjust_kernel(Adjust a) {
     }
     const int i = (n & ~3) + threadIdx.x;
     if (i < n) out[i] = one(i, x[i]);
+  } else if (HELD) {
+    const float *v = reinterpret_cast<const float *>(held);
+#pragma unroll
+    for (int j = 0; j < 4 * AHEAD; ++j) {
+      const int i = threadIdx.x + j * AT;
+      if (i < n) out[i] = one(i, v[HELD ? j : 0]);
+    }
   } else {
-#pragma unroll
-    for (int j = 0; j < AHEAD; ++j) {
-      const float *v = reinterpret_cast<const float *>(&held[j]);
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int i = threadIdx.x + (4 * j + k) * AT;
-        if (i < n) out[i] = one(i, v[k]);
-      }
+#pragma unroll 2
+    for (int i = threadIdx.x; i < n; i += 2 * AT) {        // two at once: nothing is read ahead of a store
+      const int second = i + AT < n ? i + AT : i;
+      const float v = one(i, ahead[i]), w = one(second, ahead[second]);
+      out[i] = v;
+      if (second != i) out[second] = w;
     }
   }
 }
@@ -234,17 +246,20 @@ LLM_EXPORT int llm_adjust_logits(const AdjustLogitsCall *call) {
   Adjust a{c.logits, c.out, c.ld, c.ldo, (int)c.V, 0, c.history, c.slots, c.lengths, c.ldh, (int)c.places, (int)c.longest,
            {c.repetition, (float)c.repetition_all}, {c.presence, (float)c.presence_all}, {c.frequency, (float)c.frequency_all}, c.bias, c.ld_bias,
            c.allowed, c.ld_allowed};
-  // Slices as large as still make four CTAs of 256 threads to an SM.  Few rows with long histories: CTAs of 1,024 threads, two to an SM, read a
+  // Slices as large as still make four CTAs of 256 threads to an SM; where there are more than six, of one size each: 128,256 tokens make 32 slices of
+  // 4,032, of which seven fit an SM and not six (64 rows 19.3 -> 17.3 us; 16 rows of 151,936, 4.1 to an SM, 5.9 -> 6.4: a nearly empty last one is less).  Few rows with long histories: CTAs of 1,024 threads, two to an SM, read a
   // history in a quarter of the rounds (8 rows x 128,256, 2,048 ids 4.6 -> 4.0 us, 16,384 12.9 -> 7.0; 1 row, 2,048 ids 2.7 -> 3.0, 32,768 13.1 -> 6.8).
   int slice = MOST_SLICE, wide = MOST_SLICE;
   while (slice > 1024 && (c.V + slice - 1) / slice * c.B < 4ll * sm_count()) slice /= 2;
   while (wide > 1024 && (c.V + wide / 2 - 1) / (wide / 2) * c.B <= 2ll * sm_count()) wide /= 2;
   const bool many = c.history && c.longest * c.B >= 8192 && (c.V + wide - 1) / wide * c.B <= 2ll * sm_count();
   if (many) slice = wide;
+  const long long slices = (c.V + slice - 1) / slice;
+  if (slices * c.B > 6ll * sm_count()) slice = (int)(((c.V + slices - 1) / slices + 31) / 32 * 32);
   a.slice = slice;
   const bool vec = ((uintptr_t)c.logits | (uintptr_t)c.out | (uintptr_t)c.bias) % 16 == 0 && (c.ld | c.ldo | (c.bias ? c.ld_bias : 0)) % 4 == 0;
   const dim3 grid((unsigned)((c.V + slice - 1) / slice), (unsigned)c.B);
-  const size_t smem = c.history ? (size_t)slice * sizeof(unsigned) : 0;
+  const size_t smem = (size_t)slice * sizeof(unsigned) * ((c.history ? 1 : 0) + (many ? 0 : 1));
   const cudaStream_t stream = (cudaStream_t)c.stream;
   auto kernel = vec ? (many ? adjust_kernel<true, 1024> : adjust_kernel<true, 256>) : (many ? adjust_kernel<false, 1024> : adjust_kernel<false, 256>);
   LLM_CHECK_CUDA(llm_launch(kernel, grid, dim3(many ? 1024 : 256), smem, stream, a), "adjust_logits launch");
