@@ -430,7 +430,9 @@ int dispatch_dequantize(const Fp4DequantizeCall &c) {
 // The structure is gemm_tc.cu's: W's rows are the instruction's 128 rows, the tokens its N (16 to 128); a persistent CTA to an SM with a
 // loader, an issuer and four epilogue warps, a ring of stages of 256 of K, two accumulators.  With the codes of a stage come its scales,
 // as they lie in memory; the issuer has them copied to tensor memory (tcgen05.cp, in order with the products that read
-// them) in two places in turn, behind the accumulators.
+// them) behind the accumulators.  Nothing orders a copy behind earlier products that read what was there, so every stage of the ring has its place: what
+// says that the stage is free says so of the place.  (With two places and a wait for the products of two stages ago 8 x 28,672 x 4,096 took 15.0 us
+// for 12.4.)
 constexpr int FP_THREADS = 192;
 constexpr int FP_ROWS = 128;
 
@@ -442,7 +444,7 @@ struct FpShape {
   static constexpr int STAGE_BYTES = A_BYTES + B_BYTES + 2 * SF_BYTES;
   static constexpr int STAGES = 190 * 1024 / STAGE_BYTES;
   static constexpr int SF_COLS = TILES * 8;                               // columns of tensor memory of a stage's scales
-  static constexpr int COLS = 2 * TN + 2 * SF_COLS;
+  static constexpr int COLS = 2 * TN + STAGES * SF_COLS;
   static constexpr int TMEM_COLS = COLS <= 128 ? 128 : COLS <= 256 ? 256 : 512;
   static constexpr int ROW_BYTES = 4 * TN * 4;                            // row scales of the tile's tokens, for each epilogue warp
   static constexpr size_t SMEM = 1024 + (size_t)STAGES * STAGE_BYTES + ROW_BYTES + 512;
@@ -618,7 +620,7 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
     // ------------------------------------------------------------ tensor-core issue
     const bool leader = elect_one();
     int stage = 0, iter = 0;
-    unsigned phase = 0, turn = 0;
+    unsigned phase = 0;
     bool ok = true;
     for (int tile = tile0; tile < n_tiles && ok; tile += step, ++iter) {
       const int acc = iter & 1, tok0 = tile % tok_tiles * TN;
@@ -627,14 +629,14 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
       if (!ok) break;
       tc_fence_after();
       const unsigned d_tmem = tmem_base + acc * TN;
-      for (int kb = kb0; kb < kb1; ++kb, turn ^= 1) {
+      for (int kb = kb0; kb < kb1; ++kb) {
         ok = __all_sync(0xffffffffu, mbar_wait(bar_full + 8 * stage, phase, abort_flag, status, 3));
         if (!ok) break;
         tc_fence_after();
         const unsigned a_addr = smem_u32(smem + (size_t)stage * S::STAGE_BYTES);
         const unsigned long long a_desc = smem_desc(a_addr), b_desc = smem_desc(a_addr + S::A_BYTES);
         const unsigned sf = a_addr + S::A_BYTES + S::B_BYTES;
-        const unsigned sfa = tmem_base + 2 * TN + turn * S::SF_COLS, sfb = sfa + S::TILES * 4;
+        const unsigned sfa = tmem_base + 2 * TN + stage * S::SF_COLS, sfb = sfa + S::TILES * 4;
         if (leader) {
 #pragma unroll
           for (int j = 0; j < S::TILES; ++j) {
@@ -826,7 +828,7 @@ int launch_fp4(const void *x_codes, const void *w_codes, const Fp4In &in, void *
 // products, 120 bytes a cycle where loads end at 64.  A cluster of two CTAs works on a tile of 256 tokens x 192 features (cta_group::2): each
 // brings 128 tokens and 96 features, 34 KB, and holds the sums of its tokens; the instruction has them in its lanes and the features in its
 // columns.  The CTA of even rank issues the products and the copies of scales for both; each CTA brings the scales of its tokens and of all 192
-// features.  The epilogue warps scale the sums, put boxes of 32 x 32 into buffers of their own, two in turn, and have TMA store them.  A result
+// features, in two places in turn.  The epilogue warps scale the sums, put boxes of 32 x 32 into buffers of their own, two in turn, and have TMA store them.  A result
 // whose rows do not start on 16 bytes, and the box that hangs over the last feature, are stored by the lanes themselves.
 constexpr int PR_TOKENS = 256, PR_FEATURES = 192;
 template <int FORMAT, typename TO>
@@ -993,29 +995,35 @@ fp4_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
     }
   } else if (warp == 1) {
     // ------------------------------------------------------------ products and copies of scales in both CTAs, issued by rank 0
-    const bool leader = elect_one();
     auto commit = [&](unsigned bar) {          // arrives at this barrier in both CTAs when what was issued so far is done
       asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
                    ::"r"(bar), "h"((unsigned short)3) : "memory");
     };
-    int stage = 0, iter = 0;
-    unsigned phase = 0, turn = 0;
-    bool ok = rank == 0;
-    for (int tile = first; tile < n_tiles && ok; tile += step, ++iter) {
-      const int acc = iter & 1;
-      const unsigned shift = (unsigned)(tile / tok_tiles * PR_FEATURES % 128 / 32);       // a tile may start in the middle of a scale tile
-      ok = __all_sync(0xffffffffu, mbar_wait(bar_tempty + 8 * acc, ((iter >> 1) & 1) ^ 1, abort_flag, status, 2));
-      if (!ok) break;
-      tc_fence_after();
-      const unsigned d_tmem = tmem_base + acc * PR_FEATURES;
-      for (int kb = 0; kb < n_stages; ++kb, turn ^= 1) {
-        ok = __all_sync(0xffffffffu, mbar_wait(bar_full + 8 * stage, phase, abort_flag, status, 3));
+    // One lane alone: with the warp's votes behind every wait the wait for a place cost 5 %.
+    if (elect_one() && rank == 0) {
+      int stage = 0, iter = 0, issued = 0;
+      unsigned phase = 0, turn = 0;
+      bool ok = true;
+      for (int tile = first; tile < n_tiles && ok; tile += step, ++iter) {
+        const int acc = iter & 1;
+        const unsigned shift = (unsigned)(tile / tok_tiles * PR_FEATURES % 128 / 32);     // a tile may start in the middle of a scale tile
+        ok = mbar_wait(bar_tempty + 8 * acc, ((iter >> 1) & 1) ^ 1, abort_flag, status, 2);
         if (!ok) break;
-        tc_fence_after();
-        const unsigned a_addr = smem_u32(smem + (size_t)stage * S::STAGE_BYTES), sf = a_addr + S::A_BYTES + S::B_BYTES;
-        const unsigned long long a_desc = smem_desc(a_addr), b_desc = smem_desc(a_addr + S::A_BYTES);
-        const unsigned sfa = tmem_base + 2 * PR_FEATURES + turn * S::SF_COLS, sfb = sfa + S::TILES * 4;
-        if (leader) {
+        const unsigned d_tmem = tmem_base + acc * PR_FEATURES;
+        for (int kb = 0; kb < n_stages; ++kb, turn ^= 1) {
+          // Nothing orders a copy of scales behind the products that read what was in its place: those of two stages ago have to be done.  Asked before
+          // the wait for the stage this costs nothing (8,192 cubed 219 us, without it 220), behind it 6 % (230).
+          if (issued >= 2) {
+            const int ago = stage >= 2 ? stage - 2 : stage - 2 + STAGES;
+            ok = mbar_wait(bar_empty + 8 * ago, stage >= 2 ? phase : phase ^ 1, abort_flag, status, 2);
+          }
+          issued += issued < 2;
+          ok = ok && mbar_wait(bar_full + 8 * stage, phase, abort_flag, status, 3);
+          if (!ok) break;
+          tc_fence_after();
+          const unsigned a_addr = smem_u32(smem + (size_t)stage * S::STAGE_BYTES), sf = a_addr + S::A_BYTES + S::B_BYTES;
+          const unsigned long long a_desc = smem_desc(a_addr), b_desc = smem_desc(a_addr + S::A_BYTES);
+          const unsigned sfa = tmem_base + 2 * PR_FEATURES + turn * S::SF_COLS, sfb = sfa + S::TILES * 4;
 #pragma unroll
           for (int j = 0; j < S::TILES; ++j) {
             pair_scales_to_tmem(sfa + j * 4, sf + j * SF_TILE);
@@ -1029,16 +1037,15 @@ fp4_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
                              fp4_instr(FORMAT, PR_TOKENS, PR_FEATURES, at), sfa + j * 4, sfb + j * 8 + shift, kk > 0 || kb > 0 ? 1u : 0u);
           }
           commit(bar_empty + 8 * stage);
+          if (++stage == STAGES) {
+            stage = 0;
+            phase ^= 1;
+          }
         }
-        __syncwarp();
-        if (++stage == STAGES) {
-          stage = 0;
-          phase ^= 1;
-        }
+        if (ok) commit(bar_tfull + 8 * acc);
       }
-      if (ok && leader) commit(bar_tfull + 8 * acc);
-      __syncwarp();
     }
+    __syncwarp();
     grid_dependency_wait();
   } else {
     // ------------------------------------------------------------ epilogue of this CTA's 128 tokens (warps 2 and up)
