@@ -37,6 +37,9 @@ __host__ __device__ inline long long k_stages(long long K) { return (K + STAGE_K
 __host__ __device__ inline long long code_bytes(long long K) { return (K + 31) / 32 * 16; }           // of a row
 
 // ---------------------------------------------------------------- into four bits
+// One pass: a row's values stay in registers between its maximum and its codes.  Memory bounds it (128,256 x 2,048 into nvfp4: bfloat16 96 us, 7.0 TB/s; 32-bit
+// 170 us, 7.1 TB/s) since a lane has a whole block of nvfp4, so that its scale is worked out once and no lane asks another, and products and
+// sums go in pairs; with half as many values to a lane instructions did (131 us).
 // UNIT values of a row as they lie in memory, a lane's share: a block of nvfp4, half of one of mxfp4.
 template <typename T>
 struct Unit;
@@ -100,7 +103,8 @@ template <typename T>
 __device__ __forceinline__ Unit<T> fetch_unit(const T *row, int u, int K, bool vec) {
   Unit<T> x;
   if (vec && (u + 1) * UNIT <= K) x.load(row + u * UNIT);
-  else x.gather(row + u * UNIT, K - u * UNIT);
+  else if (u * UNIT < K) x.gather(row + u * UNIT, K - u * UNIT);
+  else x = Unit<T>{};
   return x;
 }
 
@@ -158,7 +162,7 @@ template <typename T, int FORMAT>
 __device__ __forceinline__ unsigned scale_byte(unsigned top, float row_up) {
   if (FORMAT == MXFP4) return top == 0 ? 0u : (unsigned)max((int)(top >> 23) - 2, 0);       // 253 at most
   float wanted = __uint_as_float(top) * row_up;
-  if (sizeof(T) == 4) wanted = __fdiv_rn(wanted, 6.f);
+  if (sizeof(T) == 4) wanted = __fdiv_rn(fmaxf(wanted, 9.313226e-10f), 6.f);         // (see unit_codes; becomes the smallest scale either way)
   else wanted = __uint_as_float((__float_as_uint(wanted * (1.f / 6.f)) + 0x800u) & 0xfffff000u);
   const unsigned byte = __nv_cvt_float_to_fp8(wanted, __NV_SATFINITE, __NV_E4M3);
   return top == 0 ? 0u : max(byte, 1u);
@@ -166,11 +170,15 @@ __device__ __forceinline__ unsigned scale_byte(unsigned top, float row_up) {
 
 // A unit's codes.  row_up: 1 / row scale.
 //
-// nvfp4: value / row scale is exact.  The quotient by the block's scale s may be rounded before it is rounded to a code, but not across a
-// halfway point t.  32-bit values: the division's own rounding keeps the two apart (value and s t are 32-bit numbers, so they
-// differ by a step of theirs, more than half a step of the quotient).  Bfloat16 values (8 bits) and s t (4 + 3 bits) are equal or differ by 2^-8 of
-// themselves, 2^-10 or more in the quotient: value * (1 / s), which is off by 2^-21 of itself, is rounded to a multiple of 2^-13 (added to
-// 1536, whose steps these are, and taken away again), which makes it t exactly where the quotient is and leaves it on its side of t elsewhere.
+// nvfp4: a = value / row scale is exact.  What has to be told is on which side of a halfway point t the quotient a / s by the block's scale lies, or
+// that it is t.  a * (1 / s), off by 2^-21 of itself, is rounded to m, a multiple of 2^-13 (added to 1536, whose steps these are, and taken
+// away again): t is one, and where m is not t the quotient is on m's side of it, also 2^-14 further.
+//   Bfloat16 values (8 bits) and s t (4 + 3 bits) are equal or differ by 2^-8 of themselves, 2^-10 or more in the quotient: m is t exactly where the
+// quotient is.
+//   32-bit values: where m is t the sign of a - m s says it, which one instruction rounds once; m goes 2^-14 to that side.  (With divisions, which take
+// a long way round for zeros, 65,536 rows of 1,024 took 52 us, of 768 and of 1,000, in which lanes have nothing, 91 and 94.)
+// Above 0 for d > 0: 1; below: 0; 0: a half.  d is 0, or 2^-35 or more where a / s is near a halfway point.
+__device__ __forceinline__ float side(float d) { return __saturatef(fmaf(d, 6.8719476736e10f, 0.5f)); }
 template <typename T, int FORMAT>
 __device__ __forceinline__ uint2 unit_codes(const Unit<T> &x, unsigned byte, float row_up) {
   float2 v[UNIT / 2];
@@ -181,9 +189,16 @@ __device__ __forceinline__ uint2 unit_codes(const Unit<T> &x, unsigned byte, flo
 #pragma unroll
     for (int i = 0; i < UNIT / 2; ++i) v[i] = mul_two(v[i], make_float2(up, up));
   } else if (sizeof(T) == 4) {
-    const float s = byte == 0 ? 1.f : e4m3_value(byte);                // an empty block is zeros by any scale
+    const float s = byte == 0 ? 1.f : e4m3_value(byte), by = reciprocal(s);          // an empty block is zeros by any scale
 #pragma unroll
-    for (int i = 0; i < UNIT / 2; ++i) v[i] = make_float2(__fdiv_rn(v[i].x * row_up, s), __fdiv_rn(v[i].y * row_up, s));
+    for (int i = 0; i < UNIT / 2; ++i) {
+      const float2 a = mul_two(v[i], make_float2(row_up, row_up));
+      const float2 m = add_two(fma_two(a, make_float2(by, by), make_float2(1536.f, 1536.f)), make_float2(-1536.f, -1536.f));
+      const float2 d = fma_two(m, make_float2(-s, -s), a);
+      const float2 q = add_two(fma_two(make_float2(side(d.x), side(d.y)), make_float2(1.220703125e-4f, 1.220703125e-4f), m),
+                               make_float2(-6.103515625e-5f, -6.103515625e-5f));
+      v[i] = make_float2(copysignf(q.x, a.x), copysignf(q.y, a.y));
+    }
   } else {
     if (row_up > 1.7e35f) {                    // 2^117: 1 / (row scale * s) would be beyond 32 bits, the row in two steps
       const float up = power_of_two(64);
@@ -316,10 +331,14 @@ int launch_quantize(const void *x, long long ldx, const Fp4Out &o, long long row
 #define FP4_WARP(LANES, ROWS, HELD) \
   FP4_GO((fp4_quantize_warp_kernel<T, FORMAT, LANES, ROWS, HELD>), (rows + 128 / LANES * ROWS - 1) / (128 / LANES * ROWS), 128)
 #define FP4_BLOCK(THREADS, HELD) FP4_GO((fp4_quantize_block_kernel<T, FORMAT, THREADS, HELD>), rows, THREADS)
+  // us, bfloat16 into nvfp4.  Rows of up to 512 go in pairs, so that two rows' loads are on their way (128,256 x 256: 15.5, a row to a warp 35.8; 65,536 x
+  // 512: 15.2, 18.9).  Up to 2,048 a row is a warp's (128,256 x 2,048: 96.6, a block of 128 threads 135), but where rows are too few to fill the chip
+  // that way (beyond 1,024, 32-bit, 1,000 rows: 5.0, a block 4.2; bfloat16, 2,000 rows 4.4 and 4.0; 1,200 x 1,024: 2.7 and 3.0).  Longer rows: blocks as
+  // small as hold two units a thread (65,536 x 4,096: 98.8, one unit 121, four 145), and beyond those of 1,024 threads the row is read twice.
   if (n_units <= 16) FP4_WARP(16, 2, 1);
   if (n_units <= 32) FP4_WARP(32, 2, 1);
-  if (n_units <= 128 && rows <= 4 * sm_count()) FP4_BLOCK(128, 1);
   if (n_units <= 64) FP4_WARP(32, 1, 2);
+  if (n_units <= 128 && rows <= 16 * sm_count()) FP4_BLOCK(128, 1);
   if (n_units <= 128) FP4_WARP(32, 1, 4);
   if (n_units <= 256) FP4_BLOCK(128, 2);
   if (n_units <= 512) FP4_BLOCK(256, 2);
@@ -348,6 +367,8 @@ __device__ __forceinline__ void store_unit(float *p, const float (&v)[EIGHT]) {
   reinterpret_cast<float4 *>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
 }
 
+// Memory bounds it (128,256 x 2,048 of nvfp4 into bfloat16 115 us, 5.9 TB/s; three quarters of the issue slots are taken).
+//
 // A warp to four times 32 units at a time: PER of them from one row, neighbouring lanes neighbouring units, the others from the rows behind it.
 template <typename TO, int FORMAT, int PER>
 __global__ void __launch_bounds__(256)
@@ -416,6 +437,7 @@ int launch_dequantize(const Fp4DequantizeCall &c) {
                  "fp4_dequantize launch");
   return LLM_OK;
 }
+// (128,256 x 256: 18.7 us, four from one row 35.3; 65,536 x 512: 16.9, 23.2.)
 template <typename TO, int FORMAT>
 int dispatch_dequantize(const Fp4DequantizeCall &c) {
   if (c.cols <= 32 * EIGHT) return launch_dequantize<TO, FORMAT, 1>(c);
@@ -433,6 +455,9 @@ int dispatch_dequantize(const Fp4DequantizeCall &c) {
 // them) behind the accumulators.  Nothing orders a copy behind earlier products that read what was there, so every stage of the ring has its place: what
 // says that the stage is free says so of the place.  (With two places and a wait for the products of two stages ago 8 x 28,672 x 4,096 took 15.0 us
 // for 12.4.)
+//
+// Few tokens: W's bytes bound it (8 x 128,256 x 2,048: 27.4 us, 5.5 TB/s over seven rounds of tiles; 8 x 28,672 x 4,096: 12.4 us, 5.3 TB/s), and for small
+// matrices the latency of one round, which parts of K in a cluster shorten (k_parts).
 constexpr int FP_THREADS = 192;
 constexpr int FP_ROWS = 128;
 
@@ -828,8 +853,12 @@ int launch_fp4(const void *x_codes, const void *w_codes, const Fp4In &in, void *
 // products, 120 bytes a cycle where loads end at 64.  A cluster of two CTAs works on a tile of 256 tokens x 192 features (cta_group::2): each
 // brings 128 tokens and 96 features, 34 KB, and holds the sums of its tokens; the instruction has them in its lanes and the features in its
 // columns.  The CTA of even rank issues the products and the copies of scales for both; each CTA brings the scales of its tokens and of all 192
-// features, in two places in turn.  The epilogue warps scale the sums, put boxes of 32 x 32 into buffers of their own, two in turn, and have TMA store them.  A result
-// whose rows do not start on 16 bytes, and the box that hangs over the last feature, are stored by the lanes themselves.
+// features, in two places in turn.  The epilogue warps scale the sums, put boxes of 32 x 32 into buffers of their own, two in turn, and have
+// TMA store them.  A result whose rows do not start on 16 bytes, and the box that hangs over the last feature, are stored by the lanes themselves.
+//
+// 8,192 cubed: mxfp4 203 us, 5.4 PFLOP/s, nvfp4 219 us, 5.0; a stage takes 570 cycles for some 400 of products, 34 KB at 60 bytes a cycle.  2,048 x 16,384 x 2,048
+// nvfp4: 41.5 us, ten rounds of tiles of eight stages; 37 without an epilogue.  With six stages in the ring and half the buffers, or eight epilogue
+// warps, it takes the same; one SM to a tile took 242 us at 8,192 cubed.
 constexpr int PR_TOKENS = 256, PR_FEATURES = 192;
 template <int FORMAT, typename TO>
 struct PairShape {

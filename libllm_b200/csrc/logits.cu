@@ -247,8 +247,9 @@ LLM_EXPORT int llm_adjust_logits(const AdjustLogitsCall *call) {
            {c.repetition, (float)c.repetition_all}, {c.presence, (float)c.presence_all}, {c.frequency, (float)c.frequency_all}, c.bias, c.ld_bias,
            c.allowed, c.ld_allowed};
   // Slices as large as still make four CTAs of 256 threads to an SM; where there are more than six, of one size each: 128,256 tokens make 32 slices of
-  // 4,032, of which seven fit an SM and not six (64 rows 19.3 -> 17.3 us; 16 rows of 151,936, 4.1 to an SM, 5.9 -> 6.4: a nearly empty last one is less).  Few rows with long histories: CTAs of 1,024 threads, two to an SM, read a
-  // history in a quarter of the rounds (8 rows x 128,256, 2,048 ids 4.6 -> 4.0 us, 16,384 12.9 -> 7.0; 1 row, 2,048 ids 2.7 -> 3.0, 32,768 13.1 -> 6.8).
+  // 4,032, of which seven fit an SM and not six (64 rows 19.3 -> 17.3 us; 16 rows of 151,936, 4.1 to an SM, 5.9 -> 6.4: a nearly empty last one is
+  // less).  Few rows with long histories: CTAs of 1,024 threads, two to an SM, read a history in a quarter of the rounds (8 rows x 128,256, 2,048 ids
+  // 4.6 -> 4.0 us, 16,384 12.9 -> 7.0; 1 row, 2,048 ids 2.7 -> 3.0, 32,768 13.1 -> 6.8).
   int slice = MOST_SLICE, wide = MOST_SLICE;
   while (slice > 1024 && (c.V + slice - 1) / slice * c.B < 4ll * sm_count()) slice /= 2;
   while (wide > 1024 && (c.V + wide / 2 - 1) / (wide / 2) * c.B <= 2ll * sm_count()) wide /= 2;

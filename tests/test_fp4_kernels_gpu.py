@@ -61,6 +61,30 @@ def test_halves_go_to_the_even_code_under_every_scale(format, dtype):
     same_values(x, format, ops().fp4_dequantize(ops().fp4_quantize(x.to(DEV), format)))
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_the_numbers_next_to_every_border_under_every_e4m3_scale(dtype):
+    """A row of 1,536 at most has the scale 1, so that a block of 6 s at most has the scale s: every e4m3 number up to 256."""
+    borders = torch.tensor([.25, .75, 1.25, 1.75, 2.5, 3.5, 5], dtype=torch.float64)
+    scales = [m * 2.0 ** -9 for m in range(1, 8)] + [(8 + m) / 8 * 2.0 ** e for e in range(-6, 8) for m in range(8)] + [256.0]
+    blocks = [torch.zeros(16)]
+    blocks[0][3] = 1536
+    for s in scales:
+        t = (borders * s).to(dtype)                        # exact: seven bits at most
+        assert torch.equal(t.double(), borders * s)
+        bits = t.view(torch.int16 if dtype == torch.bfloat16 else torch.int32)
+        below, above = (bits - 1).view(dtype).float(), (bits + 1).view(dtype).float()
+        for near in (torch.cat([below, t.float()]), torch.cat([above, -t.float()]), torch.cat([-below, -above])):
+            block = torch.zeros(16)
+            block[0] = 6 * s
+            block[1:15] = near
+            blocks.append(block)
+    x = torch.cat(blocks)[None]
+    x = torch.cat([x, -x, x * 2.0 ** -60, x * 2.0 ** 90]).to(dtype)
+    code, scale, row = P.quantize(x, "nvfp4")
+    assert set(scale[0, 1:].flatten().tolist()) == set(scales) and row[0, 0] == 1
+    same_values(x, "nvfp4", ops().fp4_dequantize(ops().fp4_quantize(x.to(DEV), "nvfp4")))
+
+
 @pytest.mark.parametrize("format", FORMATS)
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_zeros_and_the_ends_of_the_range(format, dtype):
