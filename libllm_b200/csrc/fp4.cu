@@ -100,11 +100,36 @@ struct Unit<float> {
 };
 
 template <typename T>
-__device__ __forceinline__ Unit<T> fetch_unit(const T *row, int u, int K, bool vec) {
+__device__ __forceinline__ Unit<T> fetch_unit(const T *row, int u, int K) {
   Unit<T> x;
-  if (vec && (u + 1) * UNIT <= K) x.load(row + u * UNIT);
+  if ((u + 1) * UNIT <= K) x.load(row + u * UNIT);
   else if (u * UNIT < K) x.gather(row + u * UNIT, K - u * UNIT);
   else x = Unit<T>{};
+  return x;
+}
+
+// The units of G neighbouring lanes, u of lane 0 and those behind it, of a row that does not start on 16 bytes: lanes read neighbouring values and
+// hand them over in shared memory, 1 KB of a warp's.  (Each lane on its own, value by value: 65,536 x 2,047 142 us for 82, of 32 bits 258 for 169.)  All lanes of a warp take part.
+template <typename T, int G>
+__device__ __forceinline__ Unit<T> fetch_unit_over(const T *row, int u, int K, unsigned *stage_raw) {
+  constexpr int PASSES = sizeof(T) / 2, TURN = G / PASSES * UNIT;        // values of a turn
+  T *stage = reinterpret_cast<T *>(stage_raw) + threadIdx.x % 32 / G * TURN;
+  const int lane = threadIdx.x % G, k0 = (u - lane) * UNIT + lane;
+  Unit<T> x;
+#pragma unroll
+  for (int p = 0; p < PASSES; ++p) {
+    T v[TURN / G];
+#pragma unroll
+    for (int j = 0; j < TURN / G; ++j) {
+      const int k = k0 + p * TURN + j * G;
+      v[j] = k < K ? row[k] : T(0.f);
+    }
+    __syncwarp();
+#pragma unroll
+    for (int j = 0; j < TURN / G; ++j) stage[j * G + lane] = v[j];
+    __syncwarp();
+    if (lane / (G / PASSES) == p) x.load(stage + lane % (G / PASSES) * UNIT);
+  }
   return x;
 }
 
@@ -240,18 +265,23 @@ __device__ __forceinline__ float row_scale_of(int format, unsigned top) {
 
 // Short rows: LANES lanes to a row, ROWS rows of each such group at once, HELD units of each in a lane's registers between the row's maximum and
 // the codes.
-template <typename T, int FORMAT, int LANES, int ROWS, int HELD>
+template <typename T, int FORMAT, bool VEC, int LANES, int ROWS, int HELD>
 __global__ void __launch_bounds__(128)
-fp4_quantize_warp_kernel(const T *x, long long ldx, Fp4Out o, long long rows, int K, int n_units, int vec) {
+fp4_quantize_warp_kernel(const T *x, long long ldx, Fp4Out o, long long rows, int K, int n_units) {
   grid_dependents_launch();
   grid_dependency_wait();
   const int lane = threadIdx.x % LANES;
   const long long row0 = ((long long)blockIdx.x * (128 / LANES) + threadIdx.x / LANES) * ROWS;
+  __shared__ __align__(16) unsigned stage[VEC ? 1 : 4][VEC ? 1 : 256];
   Unit<T> held[ROWS][HELD];
 #pragma unroll
   for (int r = 0; r < ROWS; ++r)
 #pragma unroll
-    for (int i = 0; i < HELD; ++i) held[r][i] = fetch_unit(x + (row0 + r) * ldx, lane + i * LANES, row0 + r < rows ? K : 0, vec);
+    for (int i = 0; i < HELD; ++i) {
+      const T *from = x + (row0 + r) * ldx;
+      const int end = row0 + r < rows ? K : 0;
+      held[r][i] = VEC ? fetch_unit(from, lane + i * LANES, end) : fetch_unit_over<T, LANES>(from, lane + i * LANES, end, stage[VEC ? 0 : threadIdx.x / 32]);
+    }
 #pragma unroll
   for (int r = 0; r < ROWS; ++r) {
     unsigned tu[HELD], top = 0;
@@ -275,20 +305,22 @@ fp4_quantize_warp_kernel(const T *x, long long ldx, Fp4Out o, long long rows, in
 }
 
 // A block of THREADS threads to a row: HELD units of it in a thread's registers, or (HELD 0) the row read twice.
-template <typename T, int FORMAT, int THREADS, int HELD>
+template <typename T, int FORMAT, bool VEC, int THREADS, int HELD>
 __global__ void __launch_bounds__(THREADS)
-fp4_quantize_block_kernel(const T *x, long long ldx, Fp4Out o, long long rows, int K, int n_units, int vec) {
+fp4_quantize_block_kernel(const T *x, long long ldx, Fp4Out o, long long rows, int K, int n_units) {
   grid_dependents_launch();
   grid_dependency_wait();
   __shared__ unsigned tops[THREADS / 32];
+  __shared__ __align__(16) unsigned stage[VEC ? 1 : THREADS / 32][VEC ? 1 : 256];
   const int t = threadIdx.x;
   const long long row = blockIdx.x;
   const T *r = x + row * ldx;
   Unit<T> held[HELD ? HELD : 1];
   unsigned tu[HELD ? HELD : 1], top = 0;
+  auto fetch = [&](int u) { return VEC ? fetch_unit(r, u, K) : fetch_unit_over<T, 32>(r, u, K, stage[VEC ? 0 : t / 32]); };
   if (HELD) {
 #pragma unroll
-    for (int i = 0; i < HELD; ++i) held[i] = fetch_unit(r, t + i * THREADS, K, vec);
+    for (int i = 0; i < HELD; ++i) held[i] = fetch(t + i * THREADS);
 #pragma unroll
     for (int i = 0; i < HELD; ++i) {
       tu[i] = held[i].top();
@@ -296,7 +328,7 @@ fp4_quantize_block_kernel(const T *x, long long ldx, Fp4Out o, long long rows, i
     }
   } else {
 #pragma unroll 4
-    for (int u = t; u < n_units; u += THREADS) top = max(top, fetch_unit(r, u, K, vec).top());
+    for (int u = t; u < (n_units + 31) / 32 * 32; u += THREADS) top = max(top, fetch(u).top());      // whole warps
   }
   top = __reduce_max_sync(0xffffffffu, top);
   if (t % 32 == 0) tops[t / 32] = top;
@@ -310,27 +342,26 @@ fp4_quantize_block_kernel(const T *x, long long ldx, Fp4Out o, long long rows, i
     for (int i = 0; i < HELD; ++i) put_unit<T, FORMAT>(o, row, t + i * THREADS, t + i * THREADS < n_units, held[i], tu[i], row_up);
   } else {
 #pragma unroll 2
-    for (int u = t; u < (n_units + 31) / 32 * 32; u += THREADS) {      // whole warps
-      const Unit<T> v = fetch_unit(r, u, K, vec);
+    for (int u = t; u < (n_units + 31) / 32 * 32; u += THREADS) {
+      const Unit<T> v = fetch(u);
       put_unit<T, FORMAT>(o, row, u, u < n_units, v, v.top(), row_up);
     }
   }
 }
 
-template <typename T, int FORMAT>
+template <typename T, int FORMAT, bool VEC>
 int launch_quantize(const void *x, long long ldx, const Fp4Out &o, long long rows, int K, cudaStream_t stream) {
   const int n_units = (int)(k_stages(K) * (STAGE_K / UNIT));
-  const int vec = (uintptr_t)x % 16 == 0 && ldx * (long long)sizeof(T) % 16 == 0;
 #define FP4_GO(KERNEL, BLOCKS, THREADS)                                                                                                   \
   do {                                                                                                                                    \
     LLM_REQUIRE((BLOCKS) < (1ll << 31), "fp4_quantize: too many rows");                                                                  \
-    LLM_CHECK_CUDA(llm_launch(KERNEL, dim3((unsigned)(BLOCKS)), dim3(THREADS), 0, stream, (const T *)x, ldx, o, rows, K, n_units, vec),  \
+    LLM_CHECK_CUDA(llm_launch(KERNEL, dim3((unsigned)(BLOCKS)), dim3(THREADS), 0, stream, (const T *)x, ldx, o, rows, K, n_units),       \
                    "fp4_quantize launch");                                                                                               \
     return LLM_OK;                                                                                                                        \
   } while (0)
 #define FP4_WARP(LANES, ROWS, HELD) \
-  FP4_GO((fp4_quantize_warp_kernel<T, FORMAT, LANES, ROWS, HELD>), (rows + 128 / LANES * ROWS - 1) / (128 / LANES * ROWS), 128)
-#define FP4_BLOCK(THREADS, HELD) FP4_GO((fp4_quantize_block_kernel<T, FORMAT, THREADS, HELD>), rows, THREADS)
+  FP4_GO((fp4_quantize_warp_kernel<T, FORMAT, VEC, LANES, ROWS, HELD>), (rows + 128 / LANES * ROWS - 1) / (128 / LANES * ROWS), 128)
+#define FP4_BLOCK(THREADS, HELD) FP4_GO((fp4_quantize_block_kernel<T, FORMAT, VEC, THREADS, HELD>), rows, THREADS)
   // us, bfloat16 into nvfp4.  Rows of up to 512 go in pairs, so that two rows' loads are on their way (128,256 x 256: 15.5, a row to a warp 35.8; 65,536 x
   // 512: 15.2, 18.9).  Up to 2,048 a row is a warp's (128,256 x 2,048: 96.6, a block of 128 threads 135), but where rows are too few to fill the chip
   // that way (beyond 1,024, 32-bit, 1,000 rows: 5.0, a block 4.2; bfloat16, 2,000 rows 4.4 and 4.0; 1,200 x 1,024: 2.7 and 3.0).  Longer rows: blocks as
@@ -367,14 +398,19 @@ __device__ __forceinline__ void store_unit(float *p, const float (&v)[EIGHT]) {
   reinterpret_cast<float4 *>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
 }
 
-// Memory bounds it (128,256 x 2,048 of nvfp4 into bfloat16 115 us, 5.9 TB/s; three quarters of the issue slots are taken).
+// Memory bounds it (128,256 x 2,048 of nvfp4 into bfloat16 112 us, 6.0 TB/s, into 32 bits 191 us, 6.2; three quarters of the issue slots are
+// taken).  32-bit results, and rows that do not start on 16 bytes, go through shared memory, so that lanes store neighbouring values (each its own:
+// 269 us, and 65,536 x 2,047 of bfloat16 370 for 77).
 //
 // A warp to four times 32 units at a time: PER of them from one row, neighbouring lanes neighbouring units, the others from the rows behind it.
-template <typename TO, int FORMAT, int PER>
+template <typename TO, int FORMAT, bool VEC, int PER>
 __global__ void __launch_bounds__(256)
 fp4_dequantize_kernel(const unsigned char *codes, const unsigned char *scales, const float *row_scale, TO *out, long long ldo, long long rows, int K,
-                      int pieces, long long ldc, long long sf_tiles, int vec) {
+                      int pieces, long long ldc, long long sf_tiles) {
   constexpr int LANES = FORMAT == NVFP4 ? 2 : 4, ROWS = 4 / PER;
+  constexpr bool OVER = !VEC || sizeof(TO) == 4;                         // through shared memory
+  __shared__ __align__(16) float stage_raw[OVER ? 8 : 1][OVER ? 32 * EIGHT * sizeof(TO) / 4 : 1];
+  TO *stage = reinterpret_cast<TO *>(stage_raw[OVER ? threadIdx.x / 32 : 0]);
   grid_dependents_launch();
   grid_dependency_wait();
   const int lane = threadIdx.x & 31;
@@ -403,8 +439,8 @@ fp4_dequantize_kernel(const unsigned char *codes, const unsigned char *scales, c
       if (ROWS > 1 && row >= rows) break;
 #pragma unroll
       for (int i = 0; i < PER; ++i) {
-        const int u = u0 + i * 32;
-        if (u * EIGHT >= K) break;
+        const int u = u0 + i * 32, k0 = (u - lane) * EIGHT;
+        if ((OVER ? k0 : u * EIGHT) >= K) break;
         const float by = scale_value(FORMAT, byte[r * PER + i]) * rs[r];       // exact: a scale has four bits
         float v[EIGHT];
 #pragma unroll
@@ -413,36 +449,62 @@ fp4_dequantize_kernel(const unsigned char *codes, const unsigned char *scales, c
           v[2 * j] = f.x * by;
           v[2 * j + 1] = f.y * by;
         }
-        TO *p = out + row * ldo + u * EIGHT;
-        if (vec && (u + 1) * EIGHT <= K) {
-          store_unit(p, v);
+        TO *p = out + row * ldo;
+        if (OVER) {
+          __syncwarp();
+          store_unit(stage + lane * EIGHT, v);
+          __syncwarp();
+        }
+        if (VEC && OVER) {
+#pragma unroll
+          for (int j = 0; j < EIGHT / 4; ++j) {
+            const int at = (j * 32 + lane) * 4;
+            const float4 w = reinterpret_cast<const float4 *>(stage)[j * 32 + lane];
+            if (k0 + at + 4 <= K) {
+              *reinterpret_cast<float4 *>(p + k0 + at) = w;
+            } else {
+              if (k0 + at < K) p[k0 + at] = w.x;
+              if (k0 + at + 1 < K) p[k0 + at + 1] = w.y;
+              if (k0 + at + 2 < K) p[k0 + at + 2] = w.z;
+            }
+          }
+        } else if (OVER) {
+#pragma unroll
+          for (int j = 0; j < EIGHT; ++j)
+            if (k0 + j * 32 + lane < K) p[k0 + j * 32 + lane] = stage[j * 32 + lane];
+        } else if ((u + 1) * EIGHT <= K) {
+          store_unit(p + u * EIGHT, v);
         } else {
 #pragma unroll
           for (int j = 0; j < EIGHT; ++j)
-            if (u * EIGHT + j < K) p[j] = from_float<TO>(v[j]);
+            if (u * EIGHT + j < K) p[u * EIGHT + j] = from_float<TO>(v[j]);
         }
       }
     }
   }
 }
 
-template <typename TO, int FORMAT, int PER>
+template <typename TO, int FORMAT, bool VEC, int PER>
 int launch_dequantize(const Fp4DequantizeCall &c) {
   const long long K = c.cols, pieces = PER < 4 ? 1 : (K + 128 * EIGHT - 1) / (128 * EIGHT), jobs = (c.rows + 4 / PER - 1) / (4 / PER) * pieces;
   const long long blocks = (jobs + 7) / 8, most = 8ll * 4 * sm_count();
-  const int vec = (uintptr_t)c.out % 16 == 0 && c.ldo * (long long)sizeof(TO) % 16 == 0;
-  LLM_CHECK_CUDA(llm_launch(fp4_dequantize_kernel<TO, FORMAT, PER>, dim3((unsigned)(blocks < most ? blocks : most)), dim3(256), 0, (cudaStream_t)c.stream,
+  LLM_CHECK_CUDA(llm_launch(fp4_dequantize_kernel<TO, FORMAT, VEC, PER>, dim3((unsigned)(blocks < most ? blocks : most)), dim3(256), 0, (cudaStream_t)c.stream,
                             (const unsigned char *)c.codes, (const unsigned char *)c.scales, c.row_scale, (TO *)c.out, c.ldo, c.rows, (int)K, (int)pieces,
-                            code_bytes(K), k_stages(K) * stage_tiles(FORMAT), vec),
+                            code_bytes(K), k_stages(K) * stage_tiles(FORMAT)),
                  "fp4_dequantize launch");
   return LLM_OK;
 }
 // (128,256 x 256: 18.7 us, four from one row 35.3; 65,536 x 512: 16.9, 23.2.)
+template <typename TO, int FORMAT, bool VEC>
+int dispatch_dequantize_per(const Fp4DequantizeCall &c) {
+  if (c.cols <= 32 * EIGHT) return launch_dequantize<TO, FORMAT, VEC, 1>(c);
+  if (c.cols <= 64 * EIGHT) return launch_dequantize<TO, FORMAT, VEC, 2>(c);
+  return launch_dequantize<TO, FORMAT, VEC, 4>(c);
+}
 template <typename TO, int FORMAT>
 int dispatch_dequantize(const Fp4DequantizeCall &c) {
-  if (c.cols <= 32 * EIGHT) return launch_dequantize<TO, FORMAT, 1>(c);
-  if (c.cols <= 64 * EIGHT) return launch_dequantize<TO, FORMAT, 2>(c);
-  return launch_dequantize<TO, FORMAT, 4>(c);
+  const bool vec = ((uintptr_t)c.out | (unsigned long long)c.ldo * sizeof(TO)) % 16 == 0;
+  return vec ? dispatch_dequantize_per<TO, FORMAT, true>(c) : dispatch_dequantize_per<TO, FORMAT, false>(c);
 }
 
 // ---------------------------------------------------------------- the product
@@ -1256,8 +1318,15 @@ LLM_EXPORT int llm_fp4_quantize(const Fp4QuantizeCall *call) {
   if (c.rows == 0) return LLM_OK;
   const Fp4Out o{(unsigned char *)c.codes, (unsigned char *)c.scales, c.row_scale, code_bytes(c.cols), k_stages(c.cols) * stage_tiles((int)c.format)};
 #define FP4_ARGS c.x, c.ldx, o, c.rows, (int)c.cols, (cudaStream_t)c.stream
-  if (c.dtype == LLM_F32) return c.format == NVFP4 ? launch_quantize<float, NVFP4>(FP4_ARGS) : launch_quantize<float, MXFP4>(FP4_ARGS);
-  return c.format == NVFP4 ? launch_quantize<__nv_bfloat16, NVFP4>(FP4_ARGS) : launch_quantize<__nv_bfloat16, MXFP4>(FP4_ARGS);
+#define FP4_TYPE(T, FORMAT) return vec ? launch_quantize<T, FORMAT, true>(FP4_ARGS) : launch_quantize<T, FORMAT, false>(FP4_ARGS)
+  const bool vec = ((uintptr_t)c.x | (unsigned long long)c.ldx * (c.dtype == LLM_F32 ? 4 : 2)) % 16 == 0;
+  if (c.dtype == LLM_F32) {
+    if (c.format == NVFP4) FP4_TYPE(float, NVFP4);
+    FP4_TYPE(float, MXFP4);
+  }
+  if (c.format == NVFP4) FP4_TYPE(__nv_bfloat16, NVFP4);
+  FP4_TYPE(__nv_bfloat16, MXFP4);
+#undef FP4_TYPE
 #undef FP4_ARGS
 }
 
