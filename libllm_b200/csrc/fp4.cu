@@ -275,13 +275,18 @@ fp4_quantize_warp_kernel(const T *x, long long ldx, Fp4Out o, long long rows, in
   __shared__ __align__(16) unsigned stage[VEC ? 1 : 4][VEC ? 1 : 256];
   Unit<T> held[ROWS][HELD];
 #pragma unroll
-  for (int r = 0; r < ROWS; ++r)
+  for (int r = 0; r < ROWS; ++r) {
+    const T *from = x + (row0 + r) * ldx;
+    const int end = row0 + r < rows ? K : 0;
+    if (VEC && (lane + HELD * LANES - LANES + 1) * UNIT <= end) {        // asked once: in between the loads of a lane wait for one another
 #pragma unroll
-    for (int i = 0; i < HELD; ++i) {
-      const T *from = x + (row0 + r) * ldx;
-      const int end = row0 + r < rows ? K : 0;
-      held[r][i] = VEC ? fetch_unit(from, lane + i * LANES, end) : fetch_unit_over<T, LANES>(from, lane + i * LANES, end, stage[VEC ? 0 : threadIdx.x / 32]);
+      for (int i = 0; i < HELD; ++i) held[r][i].load(from + (lane + i * LANES) * UNIT);
+    } else {
+#pragma unroll
+      for (int i = 0; i < HELD; ++i)
+        held[r][i] = VEC ? fetch_unit(from, lane + i * LANES, end) : fetch_unit_over<T, LANES>(from, lane + i * LANES, end, stage[VEC ? 0 : threadIdx.x / 32]);
     }
+  }
 #pragma unroll
   for (int r = 0; r < ROWS; ++r) {
     unsigned tu[HELD], top = 0;
@@ -319,8 +324,13 @@ fp4_quantize_block_kernel(const T *x, long long ldx, Fp4Out o, long long rows, i
   unsigned tu[HELD ? HELD : 1], top = 0;
   auto fetch = [&](int u) { return VEC ? fetch_unit(r, u, K) : fetch_unit_over<T, 32>(r, u, K, stage[VEC ? 0 : t / 32]); };
   if (HELD) {
+    if (VEC && (t + HELD * THREADS - THREADS + 1) * UNIT <= K) {          // as above
 #pragma unroll
-    for (int i = 0; i < HELD; ++i) held[i] = fetch(t + i * THREADS);
+      for (int i = 0; i < HELD; ++i) held[i].load(r + (t + i * THREADS) * UNIT);
+    } else {
+#pragma unroll
+      for (int i = 0; i < HELD; ++i) held[i] = fetch(t + i * THREADS);
+    }
 #pragma unroll
     for (int i = 0; i < HELD; ++i) {
       tu[i] = held[i].top();
