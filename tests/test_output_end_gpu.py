@@ -315,3 +315,27 @@ def test_the_whole_output_end_together():
         e.synchronize()
         e.cache_check()
     assert drawn[0] == drawn[1]
+
+
+def test_the_command_line_takes_penalties_and_an_output_matrix_in_four_bits():
+    """``bin/llm generate`` draws what Model.generate draws, and something else without penalties."""
+    import os
+    import subprocess
+    from libllm_b200 import Model
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    folder, prompt = model_folder("C"), [5, 9, 2, 9]
+
+    def by_command(*flags):
+        out = subprocess.run([os.path.join(root, "bin", "llm"), "generate", "-m", folder, "--prompt-ids", ",".join(map(str, prompt)), "--max-new-tokens", "24",
+                              "--temperature", "0", "--dtype", "float32", "--no-stop", "--max-tokens", "2048", *flags], capture_output=True, text=True, timeout=600)
+        assert out.returncode == 0, out.stderr
+        return [int(t) for t in out.stdout.strip().splitlines()[-1].split(",")]
+
+    m = Model(folder, dtype="float32", max_tokens=2048, head="nvfp4", track_history=True)
+    want = [m.generate([prompt], 24, temperature=0.0, stop_token_ids=[], **kw)[0]
+            for kw in ({}, dict(repetition_penalty=1.5, presence_penalty=0.5, frequency_penalty=0.25))]
+    assert want[0] != want[1]
+    assert by_command("--head", "nvfp4") == want[0]
+    assert by_command("--head", "nvfp4", "--repetition-penalty", "1.5", "--presence-penalty", "0.5", "--frequency-penalty", "0.25") == want[1]
+    bad = subprocess.run([os.path.join(root, "bin", "llm"), "generate", "-m", folder, "--prompt-ids", "1,2", "--head", "fp4"], capture_output=True, text=True, timeout=600)
+    assert bad.returncode != 0 and "fp4" in bad.stderr
