@@ -42,6 +42,23 @@ def test_values_are_the_nearest(format, dtype, rows, cols):
 
 @pytest.mark.parametrize("format", FORMATS)
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("rows,cols", [(40, 130), (40, 300), (40, 777), (7, 1501), (2500, 1501), (3, 2600), (3, 5001), (3, 9001), (3, 20001), (2, 33000)])
+def test_rows_that_start_between_16_bytes(format, dtype, rows, cols):
+    """Read from, and brought back to, columns 1 and on of a wider tensor, whose border keeps what it had."""
+    wide = rows_like(rows, cols + 2, rows + cols, dtype).to(DEV)
+    x = wide[:, 1:cols + 1]
+    q = ops().fp4_quantize(x, format)
+    ref = ops().fp4_quantize(x.contiguous(), format)                    # (scales behind the last row are nobody's)
+    assert torch.equal(q.codes, ref.codes) and torch.equal(q.row_scale, ref.row_scale)
+    for to in (torch.float32, torch.bfloat16):
+        back = torch.full((rows, cols + 2), 7.0, dtype=to, device=DEV)
+        ops().fp4_dequantize(q, out=back[:, 1:cols + 1])
+        same_values(x.cpu(), format, back[:, 1:cols + 1])
+        assert (back[:, 0] == 7).all() and (back[:, -1] == 7).all()
+
+
+@pytest.mark.parametrize("format", FORMATS)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_halves_go_to_the_even_code_under_every_scale(format, dtype):
     """Values at, just below and just above every border, under all the scales that the format's blocks can have."""
     borders = torch.tensor([.25, .75, 1.25, 1.75, 2.5, 3.5, 5], dtype=torch.float64)
