@@ -925,12 +925,14 @@ int launch_fp4(const void *x_codes, const void *w_codes, const Fp4In &in, void *
 // products, 120 bytes a cycle where loads end at 64.  A cluster of two CTAs works on a tile of 256 tokens x 192 features (cta_group::2): each
 // brings 128 tokens and 96 features, 34 KB, and holds the sums of its tokens; the instruction has them in its lanes and the features in its
 // columns.  The CTA of even rank issues the products and the copies of scales for both; each CTA brings the scales of its tokens and of all 192
-// features, in two places in turn.  The epilogue warps scale the sums, put boxes of 32 x 32 into buffers of their own, two in turn, and have
-// TMA store them.  A result whose rows do not start on 16 bytes, and the box that hangs over the last feature, are stored by the lanes themselves.
+// features, in two places in turn.  The epilogue warps scale the sums, put boxes of 32 tokens x 128 bytes into buffers of their own and have TMA store
+// them (a result whose rows do not start on 16 bytes, and the box that hangs over the last feature, the lanes store from there, row by row: 1,000 x
+// 1,999 x 1,500 9.5 us, each lane a token's row 35).  With 64 bytes to a box, twice the fences, 2,048 x 16,384 x 2,048 took 41.5 us for 37, and the rows'
+// scales, loaded a tile ahead, are part of that.
 //
-// 8,192 cubed: mxfp4 203 us, 5.4 PFLOP/s, nvfp4 219 us, 5.0; a stage takes 570 cycles for some 400 of products, 34 KB at 60 bytes a cycle.  2,048 x 16,384 x 2,048
-// nvfp4: 41.5 us, ten rounds of tiles of eight stages; 37 without an epilogue.  With six stages in the ring and half the buffers, or eight epilogue
-// warps, it takes the same; one SM to a tile took 242 us at 8,192 cubed.
+// 8,192 cubed: mxfp4 205 us, 5.4 PFLOP/s, nvfp4 220 us, 5.0; a stage takes 570 cycles for some 400 of products, 34 KB at 60 bytes a cycle.  2,048 x 16,384 x
+// 2,048 nvfp4: 36.7 us (3.7 PFLOP/s), ten rounds of tiles of eight stages; with one stage to a tile 23, the epilogue's time, which hides behind eight stages
+// and no less.  One SM to a tile took 242 us at 8,192 cubed; six stages in the ring, and eight epilogue warps for twelve, change nothing.
 constexpr int PR_TOKENS = 256, PR_FEATURES = 192;
 template <int FORMAT, typename TO>
 struct PairShape {
@@ -941,9 +943,10 @@ struct PairShape {
   static constexpr int SHARES = sizeof(TO) == 4 ? 2 : 3, SHARE = PR_FEATURES / SHARES;    // epilogue warps to a quarter of the lanes; their features
   static constexpr int WARPS = 4 * SHARES, THREADS = 64 + 32 * WARPS;
   static constexpr int SF_COLS = TILES * 12;                             // columns of a stage's scales: 4 of a tile for the tokens, 8 for the features
-  static constexpr int OUT_BYTES = 32 * 32 * (int)sizeof(TO);            // 32 tokens x 32 features on their way out
+  static constexpr int BOX = 128 / (int)sizeof(TO), BOXES = SHARE / BOX, BUFFERS = BOXES > 1 ? 2 : 1;
+  static constexpr int OUT_BYTES = 32 * 128;                             // 32 tokens x BOX features on their way out
   static constexpr int ROW_BYTES = WARPS * SHARE * 4;       // row scales of its features, for each epilogue warp
-  static constexpr size_t SMEM = 1024 + (size_t)STAGES * STAGE_BYTES + 2 * WARPS * OUT_BYTES + ROW_BYTES + 256;
+  static constexpr size_t SMEM = 1024 + (size_t)STAGES * STAGE_BYTES + BUFFERS * WARPS * OUT_BYTES + ROW_BYTES + 256;
   static_assert(STAGE_BYTES % 1024 == 0 && 2 * PR_FEATURES + 2 * SF_COLS <= 512, "a stage's parts do not fit");
 };
 __device__ __forceinline__ void pair_load(unsigned dst, const CUtensorMap *map, int x, int y, unsigned bar) {
@@ -971,26 +974,20 @@ __device__ __forceinline__ void pair_mma(unsigned d, unsigned long long a, unsig
         "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n}"
         ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate) : "memory");
 }
-// 16 of a row's 32 values into the box that TMA stores, swizzled as it takes them: rows of 128 bytes, 16-byte pieces in the order piece ^ row % 8; or
-// (bfloat16) of 64 bytes, piece ^ row / 2 % 4.
-__device__ __forceinline__ void put16(unsigned box, int row, int half, const float (&v)[16], float) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(box + row * 128 + (((half * 4 + i) ^ (row & 7)) << 4)), "f"(v[4 * i]),
-                 "f"(v[4 * i + 1]), "f"(v[4 * i + 2]), "f"(v[4 * i + 3]) : "memory");
+// 16 bytes of a row of 128, the values from v on, into the box that TMA stores, swizzled as it takes them: piece ^ row % 8.
+__device__ __forceinline__ void put_piece(unsigned box, int row, int piece, const float *v, float) {
+  asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(box + row * 128 + ((piece ^ (row & 7)) << 4)), "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3])
+               : "memory");
 }
-__device__ __forceinline__ void put16(unsigned box, int row, int half, const float (&v)[16], __nv_bfloat16) {
+__device__ __forceinline__ void put_piece(unsigned box, int row, int piece, const float *v, __nv_bfloat16) {
+  unsigned w[4];
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    unsigned w[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const __nv_bfloat162 h = __floats2bfloat162_rn(v[8 * i + 2 * j], v[8 * i + 2 * j + 1]);
-      w[j] = *reinterpret_cast<const unsigned *>(&h);
-    }
-    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(box + row * 64 + (((half * 2 + i) ^ (row >> 1 & 3)) << 4)), "r"(w[0]), "r"(w[1]),
-                 "r"(w[2]), "r"(w[3]) : "memory");
+  for (int j = 0; j < 4; ++j) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
+    w[j] = *reinterpret_cast<const unsigned *>(&h);
   }
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(box + row * 128 + ((piece ^ (row & 7)) << 4)), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3])
+               : "memory");
 }
 
 template <int FORMAT, typename TO>
@@ -1003,7 +1000,7 @@ fp4_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
   extern __shared__ unsigned char smem_raw[];
   unsigned char *smem = (unsigned char *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   unsigned char *out_raw = smem + (size_t)STAGES * S::STAGE_BYTES;
-  float *row_raw = (float *)(out_raw + 2 * S::WARPS * S::OUT_BYTES);
+  float *row_raw = (float *)(out_raw + S::BUFFERS * S::WARPS * S::OUT_BYTES);
   unsigned long long *bars = (unsigned long long *)((unsigned char *)row_raw + S::ROW_BYTES);
   const unsigned bar_full = smem_u32(bars), bar_empty = smem_u32(bars + STAGES);
   const unsigned bar_tfull = smem_u32(bars + 2 * STAGES), bar_tempty = smem_u32(bars + 2 * STAGES + 2);
@@ -1152,63 +1149,98 @@ fp4_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
     // ------------------------------------------------------------ epilogue of this CTA's 128 tokens (warps 2 and up)
     grid_dependency_wait();
     const int quarter = warp & 3, from = (warp - 2) / 4 * S::SHARE;        // the lanes of tensor memory the warp may read; its first feature
-    const unsigned box0 = smem_u32(out_raw) + (unsigned)(warp - 2) * 2 * S::OUT_BYTES;
+    const unsigned box0 = smem_u32(out_raw) + (unsigned)(warp - 2) * S::BUFFERS * S::OUT_BYTES;
     float *rows = row_raw + (warp - 2) * S::SHARE;
     int iter = 0;
     unsigned turn = 0;
+    // The rows' scales, a tile ahead: from memory at each use they cost more than the rest of the epilogue.
+    float next_x = 0.f, next_w[S::SHARE / 32];
+    auto fetch = [&](int tile) {
+      const int f0 = tile / tok_tiles * PR_FEATURES + from + lane, t0 = tile % tok_tiles * PR_TOKENS + (int)rank * 128 + quarter * 32 + lane;
+      next_x = t0 < M ? x_row[t0] : 1.f;
+#pragma unroll
+      for (int i = 0; i < S::SHARE / 32; ++i) next_w[i] = f0 + i * 32 < N ? w_row[f0 + i * 32] : 1.f;
+    };
+    if (first < n_tiles) fetch(first);
     for (int tile = first; tile < n_tiles; tile += step, ++iter) {
       const int acc = iter & 1, f0 = tile / tok_tiles * PR_FEATURES + from;
       const int tok0 = tile % tok_tiles * PR_TOKENS + (int)rank * 128 + quarter * 32;
-      // the rows' scales, while the products run: from memory at each use they cost more than the rest of the epilogue
-      const float rx = tok0 + lane < M ? x_row[tok0 + lane] : 0.f;
+      const float rx = next_x;
       __syncwarp();
-      bool near = near_one(rx) || tok0 + lane >= M;
+      bool near = near_one(rx);
 #pragma unroll
-      for (int i = lane; i < S::SHARE; i += 32) {
-        const float r = f0 + i < N ? w_row[f0 + i] : 1.f;
-        near = near && near_one(r);
-        rows[i] = r;
+      for (int i = 0; i < S::SHARE / 32; ++i) {
+        near = near && near_one(next_w[i]);
+        rows[i * 32 + lane] = next_w[i];
       }
       near = __all_sync(0xffffffffu, near);
       __syncwarp();
+      if (tile + step < n_tiles) fetch(tile + step);
       if (!__all_sync(0xffffffffu, mbar_wait(bar_tfull + 8 * acc, (iter >> 1) & 1, abort_flag, status, 4))) break;
       tc_fence_after();
       const unsigned taddr = tmem_base + ((unsigned)(quarter * 32) << 16) + (unsigned)(acc * PR_FEATURES + from);
 #pragma unroll 1
-      for (int s0 = 0; s0 < S::SHARE && f0 + s0 < N && tok0 < M; s0 += 32, turn ^= 1) {
+      for (int b = 0; b < S::BOXES; ++b) {
+        const int s0 = b * S::BOX;
+        const bool there = f0 + s0 < N && tok0 < M;
+        constexpr int HALVES = S::BOX / 32, PIECE = 16 / (int)sizeof(TO);                 // 32 features at a time, the next on their way
+        const bool last = b == S::BOXES - 1;
         const unsigned box = box0 + turn * S::OUT_BYTES;
-        float a[16], b[16];
-        tc_ld16_issue(taddr + s0, a);
-        tc_ld16_issue(taddr + s0 + 16, b);
-        tc_ld_wait();
-        tc_ld_ready(a);
-        tc_ld_ready(b);
-        if (near) {
-#pragma unroll
-          for (int i = 0; i < 16; i += 4) {
-            const float4 r = *reinterpret_cast<const float4 *>(rows + s0 + i), q = *reinterpret_cast<const float4 *>(rows + s0 + 16 + i);
-            a[i] = a[i] * r.x * rx;
-            a[i + 1] = a[i + 1] * r.y * rx;
-            a[i + 2] = a[i + 2] * r.z * rx;
-            a[i + 3] = a[i + 3] * r.w * rx;
-            b[i] = b[i] * q.x * rx;
-            b[i + 1] = b[i + 1] * q.y * rx;
-            b[i + 2] = b[i + 2] * q.z * rx;
-            b[i + 3] = b[i + 3] * q.w * rx;
+        if (S::BUFFERS == 2) turn ^= 1;
+        float v[HALVES][32];
+        auto load = [&](int h) {
+          tc_ld16_issue(taddr + s0 + h * 32, *reinterpret_cast<float (*)[16]>(v[h]));
+          tc_ld16_issue(taddr + s0 + h * 32 + 16, *reinterpret_cast<float (*)[16]>(v[h] + 16));
+        };
+        auto loaded = [&](int h) {
+          tc_ld_wait();
+          tc_ld_ready(*reinterpret_cast<float (*)[16]>(v[h]));
+          tc_ld_ready(*reinterpret_cast<float (*)[16]>(v[h] + 16));
+        };
+        if (there) {
+          load(0);
+          if (lane == 0) {                     // the box's last store has read it
+            if (S::BUFFERS == 2) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+            else asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
           }
-        } else {
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            a[i] = scaled_far(a[i], rows[s0 + i], rx);
-            b[i] = scaled_far(b[i], rows[s0 + 16 + i], rx);
-          }
-        }
-        // what hangs over the last column is stored lane by lane: TMA would round its end up to 16 bytes, into what is not ours
-        if (by_tma && f0 + s0 + 32 <= N) {
-          if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");       // the box's last store has read it
           __syncwarp();
-          put16(box, lane, 0, a, TO());
-          put16(box, lane, 1, b, TO());
+        }
+#pragma unroll
+        for (int h = 0; h < HALVES; ++h) {
+          if (there) {
+            loaded(h);
+            if (h + 1 < HALVES) load(h + 1);
+          }
+          // The sums are in registers: the accumulator is free.  Where nobody waits for it this is left out: it takes half a microsecond (a fence over
+          // the cluster), 5 % of a product of one round of tiles.
+          if (last && h == HALVES - 1 && tile + 2 * step < n_tiles) {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0)
+              asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(in_cta(bar_tempty + 8 * acc, 0)) : "memory");
+          }
+          if (!there) continue;
+          if (near) {
+#pragma unroll
+            for (int i = 0; i < 32; i += 4) {
+              const float4 w = *reinterpret_cast<const float4 *>(rows + s0 + h * 32 + i);
+              float *p = &v[h][i];
+              p[0] = p[0] * w.x * rx;
+              p[1] = p[1] * w.y * rx;
+              p[2] = p[2] * w.z * rx;
+              p[3] = p[3] * w.w * rx;
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[h][i] = scaled_far(v[h][i], rows[s0 + h * 32 + i], rx);
+          }
+#pragma unroll
+          for (int i = 0; i < 32 / PIECE; ++i) put_piece(box, lane, h * (32 / PIECE) + i, &v[h][i * PIECE], TO());
+        }
+        if (!there) continue;
+        // what hangs over the last column the lanes store, as they do all of a result whose rows do not start on 16 bytes: TMA would round its end
+        // up to 16 bytes, into what is not ours
+        if (by_tma && f0 + s0 + S::BOX <= N) {
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
           __syncwarp();
           if (lane == 0) {
@@ -1216,20 +1248,18 @@ fp4_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
                          ::"l"(&map_out), "r"(f0 + s0), "r"(tok0), "r"(box) : "memory");
             asm volatile("cp.async.bulk.commit_group;" ::: "memory");
           }
-        } else if (tok0 + lane < M) {
-          TO *p = out + (size_t)(tok0 + lane) * ldo + f0 + s0;
-          const int n = N - f0 - s0;
+        } else {
+          __syncwarp();
+          const TO *from_box = reinterpret_cast<const TO *>(out_raw + (box - smem_u32(out_raw)));
+          const int n = min(N - f0 - s0, S::BOX), m = min(M - tok0, 32);
+          TO *p = out + (size_t)tok0 * ldo + f0 + s0;
+          for (int t = 0; t < m; ++t, p += ldo)
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            if (i < n) p[i] = from_float<TO>(a[i]);
-            if (16 + i < n) p[16 + i] = from_float<TO>(b[i]);
-          }
+            for (int i = lane; i < S::BOX; i += 32)
+              if (i < n) p[i] = from_box[t * S::BOX + ((i / PIECE ^ (t & 7)) * PIECE) + i % PIECE];
+          __syncwarp();
         }
       }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0)
-        asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(in_cta(bar_tempty + 8 * acc, 0)) : "memory");
     }
     if (by_tma && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     __syncwarp();
@@ -1260,16 +1290,16 @@ int get_scale_map(const void *scales, long long rows, long long K, int format, C
   LLM_REQUIRE(r == CUDA_SUCCESS, "tensor map: cuTensorMapEncodeTiled failed (%d) for scales of %lld x %lld", (int)r, rows, K);
   return LLM_OK;
 }
-// A map over the result: boxes of 32 x 32 values, swizzled over their rows (put16); rows behind the last are not stored.
+// A map over the result: boxes of 32 rows of 128 bytes, swizzled (put_piece); rows behind the last are not stored.
 int get_out_map(void *out, long long M, long long N, long long ldo, bool f32, CUtensorMap *map) {
   EncodeTiledFn fn = encode_fn();
   LLM_REQUIRE(fn != nullptr, "tensor map: the driver does not offer cuTensorMapEncodeTiled");
   const cuuint64_t dims[2] = {(cuuint64_t)N, (cuuint64_t)M};
   const cuuint64_t strides[1] = {(cuuint64_t)ldo * (f32 ? 4 : 2)};
-  const cuuint32_t box[2] = {32, 32};
+  const cuuint32_t box[2] = {f32 ? 32u : 64u, 32};
   const cuuint32_t elem[2] = {1, 1};
   const CUresult r = fn(map, f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, out, dims, strides, box, elem,
-                        CU_TENSOR_MAP_INTERLEAVE_NONE, f32 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   LLM_REQUIRE(r == CUDA_SUCCESS, "tensor map: cuTensorMapEncodeTiled failed (%d) for a result of %lld x %lld", (int)r, M, N);
   return LLM_OK;
 }
