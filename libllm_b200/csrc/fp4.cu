@@ -109,7 +109,8 @@ __device__ __forceinline__ Unit<T> fetch_unit(const T *row, int u, int K) {
 }
 
 // The units of G neighbouring lanes, u of lane 0 and those behind it, of a row that does not start on 16 bytes: lanes read neighbouring values and
-// hand them over in shared memory, 1 KB of a warp's.  (Each lane on its own, value by value: 65,536 x 2,047 142 us for 82, of 32 bits 258 for 169.)  All lanes of a warp take part.
+// hand them over in shared memory, 1 KB of a warp's.  (Each lane on its own, value by value: 65,536 x 2,047 142 us for 82, of 32 bits 258 for
+// 169.)  All lanes of a warp take part.
 template <typename T, int G>
 __device__ __forceinline__ Unit<T> fetch_unit_over(const T *row, int u, int K, unsigned *stage_raw) {
   constexpr int PASSES = sizeof(T) / 2, TURN = G / PASSES * UNIT;        // values of a turn
@@ -931,8 +932,8 @@ int launch_fp4(const void *x_codes, const void *w_codes, const Fp4In &in, void *
 // scales, loaded a tile ahead, are part of that.
 //
 // 8,192 cubed: mxfp4 205 us, 5.4 PFLOP/s, nvfp4 220 us, 5.0; a stage takes 570 cycles for some 400 of products, 34 KB at 60 bytes a cycle.  2,048 x 16,384 x
-// 2,048 nvfp4: 36.7 us (3.7 PFLOP/s), ten rounds of tiles of eight stages; with one stage to a tile 23, the epilogue's time, which hides behind eight stages
-// and no less.  One SM to a tile took 242 us at 8,192 cubed; six stages in the ring, and eight epilogue warps for twelve, change nothing.
+// 2,048 nvfp4: 37 us (3.7 PFLOP/s), ten rounds of tiles of eight stages; with one stage to a tile 22, the epilogue's time, which hides behind eight stages
+// and no fewer.  One SM to a tile took 242 us at 8,192 cubed; six stages in the ring, and eight epilogue warps for twelve, change nothing.
 constexpr int PR_TOKENS = 256, PR_FEATURES = 192;
 template <int FORMAT, typename TO>
 struct PairShape {
@@ -1253,10 +1254,22 @@ fp4_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
           const TO *from_box = reinterpret_cast<const TO *>(out_raw + (box - smem_u32(out_raw)));
           const int n = min(N - f0 - s0, S::BOX), m = min(M - tok0, 32);
           TO *p = out + (size_t)tok0 * ldo + f0 + s0;
-          for (int t = 0; t < m; ++t, p += ldo)
+          if (by_tma) {                        // rows start on 16 bytes
 #pragma unroll
-            for (int i = lane; i < S::BOX; i += 32)
-              if (i < n) p[i] = from_box[t * S::BOX + ((i / PIECE ^ (t & 7)) * PIECE) + i % PIECE];
+            for (int i = 0; i < 8; ++i) {
+              const int t = i * 4 + lane / 8, at = lane % 8 * PIECE;
+              const TO *q = from_box + t * S::BOX + (lane % 8 ^ (t & 7)) * PIECE;
+              TO *to = p + t * ldo + at;
+              if (t < m && at + PIECE <= n) *reinterpret_cast<float4 *>(to) = *reinterpret_cast<const float4 *>(q);
+              else if (t < m)
+                for (int k = 0; at + k < n; ++k) to[k] = q[k];
+            }
+          } else {
+            for (int t = 0; t < m; ++t, p += ldo)
+#pragma unroll
+              for (int i = lane; i < S::BOX; i += 32)
+                if (i < n) p[i] = from_box[t * S::BOX + ((i / PIECE ^ (t & 7)) * PIECE) + i % PIECE];
+          }
           __syncwarp();
         }
       }

@@ -237,6 +237,24 @@ def test_product_into_rows_of_a_wider_result(format, M, dtype):
 
 
 @pytest.mark.parametrize("format", FORMATS)
+@pytest.mark.parametrize("M,N", [(300, 4099), (1301, 1000), (513, 2560)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_prompts_into_rows_of_a_wider_result(format, M, N, dtype):
+    """Tiles of two SMs, whose result leaves by TMA where rows start on 16 bytes: whatever hangs over the last token or feature stays as it was."""
+    o = ops()
+    x, w = rows_like(M, 300, 1), rows_like(N, 300, 2)
+    qx, qw = o.fp4_quantize(x.to(DEV), format), o.fp4_quantize(w.to(DEV), format)
+    a, b = P.values(x, format), P.values(w, format)
+    ref = a @ b.T
+    tol = a.abs() @ b.abs().T * 300 * 2.0 ** -23 + (ref.abs() * 2.0 ** -8 if dtype == torch.bfloat16 else 0)     # as check_product
+    for at, wide in ((7, N + 21), (8, (N + 39) // 8 * 8), (8, N + 14), (0, N)):
+        out = torch.full((2 * M, wide), 3.0, device=DEV, dtype=dtype)
+        o.fp4_gemm(qx, qw, out=out[::2, at:at + N])
+        assert ((out[::2, at:at + N].double().cpu() - ref).abs() <= tol).all()
+        assert (out[1::2] == 3).all() and (out[:, :at] == 3).all() and (out[:, at + N:] == 3).all()
+
+
+@pytest.mark.parametrize("format", FORMATS)
 def test_a_tokens_result_does_not_hang_on_the_others(format):
     o = ops()
     x, w = rows_like(250, 700, 1).to(DEV), rows_like(300, 700, 2).to(DEV)
