@@ -513,32 +513,23 @@ def _fp4_layout(rows: int, cols: int, format: str):
 class Fp4Matrix:
     """A matrix [rows, cols] in four bits (csrc/fp4.cu says what lies where): codes, block scales and row scales in one piece of device
     memory.  ``fp4_quantize`` makes one or fills one again."""
-    __slots__ = ("rows", "cols", "format", "data", "_layout")
+    __slots__ = ("rows", "cols", "format", "data")
 
     def __init__(self, rows: int, cols: int, format: str = "nvfp4", device="cuda"):
-        self._layout = layout = _fp4_layouts.get((rows, cols, format)) or _fp4_layout(rows, cols, format)
         self.rows = rows
         self.cols = cols
         self.format = format
-        self.data = torch.empty(layout[4], dtype=torch.uint8, device=device)
+        self.data = torch.empty(self._layout[4], dtype=torch.uint8, device=device)
 
-    @classmethod
-    def _of(cls, data: torch.Tensor, rows: int, cols: int, format: str) -> "Fp4Matrix":
-        q = cls.__new__(cls)
-        q._layout = _fp4_layouts.get((rows, cols, format)) or _fp4_layout(rows, cols, format)
-        q.rows = rows
-        q.cols = cols
-        q.format = format
-        q.data = data
-        return q
+    @property
+    def _layout(self):
+        return _fp4_layouts.get((self.rows, self.cols, self.format)) or _fp4_layout(self.rows, self.cols, self.format)
 
     def check(self) -> None:
         """The memory is still what rows, cols and format need (all of them can be set)."""
-        d = self.data
-        if self._layout is not _fp4_layouts.get((self.rows, self.cols, self.format)):
-            self._layout = _fp4_layout(self.rows, self.cols, self.format)
-        if d.dtype != torch.uint8 or d.dim() != 1 or not d.is_contiguous() or d.size(0) != self._layout[4]:
-            raise InvalidArgError(f"fp4: {self.format} [{self.rows}, {self.cols}] lies in {self._layout[4]} contiguous bytes, data is "
+        d, size = self.data, self._layout[4]
+        if d.dtype != torch.uint8 or d.dim() != 1 or not d.is_contiguous() or d.size(0) != size:
+            raise InvalidArgError(f"fp4: {self.format} [{self.rows}, {self.cols}] lies in {size} contiguous bytes, data is "
                                   f"{str(d.dtype).replace('torch.', '')} {list(d.shape)}")
 
     @property
@@ -564,6 +555,7 @@ class Fp4Matrix:
         return self.data[self._layout[3]:].view(torch.float32)
 
 
+_new_fp4_matrix = Fp4Matrix.__new__
 # csrc/fp4.h: Fp4QuantizeCall, Fp4DequantizeCall, Fp4GemmCall
 _pack_fp4_quantize, _pack_fp4_dequantize = struct.Struct("@qPqPPPqqqP").pack, struct.Struct("@PPPqPqqqqP").pack
 _pack_fp4_gemm = struct.Struct("@PPPPPPqPqqqqqqPP").pack
@@ -584,11 +576,15 @@ def fp4_quantize(x: torch.Tensor, format: str = "nvfp4", out: Optional[Fp4Matrix
     """x [rows, cols] (bfloat16 or float32, any row stride) in four bits.  nvfp4: blocks of 16 along a row with e4m3 scales and a power of two
     per row; mxfp4: blocks of 32 with powers of two.  A code is the nearest one, halves go to the even code, what is too large becomes the
     largest.  A row that holds a NaN or an infinity becomes NaN throughout.  ``out``: a matrix of the same shape and format to fill."""
-    if out is None and format in FP4_FORMATS:
-        data = (_quick.get("fp4_quantize") or _quick_call("fp4", "fp4_quantize", x))(x, FP4_FORMATS[format])
+    if out is None:
+        data = (_quick.get("fp4_quantize") or _quick_call("fp4", "fp4_quantize", x))(x, FP4_FORMATS.get(format))
         if data is not None:
             _launched("fp4", "fp4_quantize", data)
-            return Fp4Matrix._of(data, *x.shape, format)
+            q = _new_fp4_matrix(Fp4Matrix)
+            q.rows, q.cols = x.shape
+            q.format = format
+            q.data = data
+            return q
     shape, dt = x.shape, _DT.get(x.dtype)
     if len(shape) != 2:
         raise InvalidArgError("fp4_quantize: x is [rows, cols]")
@@ -619,7 +615,7 @@ def fp4_dequantize(q: Fp4Matrix, dtype: torch.dtype = torch.float32, out: Option
     their range; an nvfp4 scale that was rounded up may take a value within 3 % of the largest number beyond it)."""
     dt, rows, cols = dtype_code(dtype if out is None else out.dtype), q.rows, q.cols
     if out is None:
-        values = (_quick.get("fp4_dequantize") or _quick_call("fp4", "fp4_dequantize", q.data))(q.data, rows, cols, q._layout[0], dt)
+        values = (_quick.get("fp4_dequantize") or _quick_call("fp4", "fp4_dequantize", q.data))(q.data, rows, cols, FP4_FORMATS.get(q.format), dt)
         if values is not None:
             _launched("fp4", "fp4_dequantize", values)
             return values
@@ -652,7 +648,7 @@ def fp4_gemm(x: Fp4Matrix, w: Fp4Matrix, out: Optional[torch.Tensor] = None, out
     word = 0 if device < 0 else _status_words.get(device) or _status_word(wd.device)
     if out is None:
         dt = dtype_code(out_dtype)
-        result = (_quick.get("fp4_gemm") or _quick_call("fp4", "fp4_gemm", wd))(xd, wd, M, N, x.cols, x._layout[0], dt, word)
+        result = (_quick.get("fp4_gemm") or _quick_call("fp4", "fp4_gemm", wd))(xd, wd, M, N, x.cols, FP4_FORMATS.get(x.format), dt, word)
         if result is not None:
             _launched("fp4", "fp4_gemm", result)
             return result
