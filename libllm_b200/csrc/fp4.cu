@@ -1184,22 +1184,11 @@ fp4_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
       for (int b = 0; b < S::BOXES; ++b) {
         const int s0 = b * S::BOX;
         const bool there = f0 + s0 < N && tok0 < M;
-        constexpr int HALVES = S::BOX / 32, PIECE = 16 / (int)sizeof(TO);                 // 32 features at a time, the next on their way
+        constexpr int HALVES = S::BOX / 32, PIECE = 16 / (int)sizeof(TO);                 // 32 features at a time
         const bool last = b == S::BOXES - 1;
         const unsigned box = box0 + turn * S::OUT_BYTES;
         if (S::BUFFERS == 2) turn ^= 1;
-        float v[HALVES][32];
-        auto load = [&](int h) {
-          tc_ld16_issue(taddr + s0 + h * 32, *reinterpret_cast<float (*)[16]>(v[h]));
-          tc_ld16_issue(taddr + s0 + h * 32 + 16, *reinterpret_cast<float (*)[16]>(v[h] + 16));
-        };
-        auto loaded = [&](int h) {
-          tc_ld_wait();
-          tc_ld_ready(*reinterpret_cast<float (*)[16]>(v[h]));
-          tc_ld_ready(*reinterpret_cast<float (*)[16]>(v[h] + 16));
-        };
         if (there) {
-          load(0);
           if (lane == 0) {                     // the box's last store has read it
             if (S::BUFFERS == 2) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
             else asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
@@ -1208,9 +1197,13 @@ fp4_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
         }
 #pragma unroll
         for (int h = 0; h < HALVES; ++h) {
+          float a[16], c[16];
           if (there) {
-            loaded(h);
-            if (h + 1 < HALVES) load(h + 1);
+            tc_ld16_issue(taddr + s0 + h * 32, a);
+            tc_ld16_issue(taddr + s0 + h * 32 + 16, c);
+            tc_ld_wait();
+            tc_ld_ready(a);
+            tc_ld_ready(c);
           }
           // The sums are in registers: the accumulator is free.  Where nobody waits for it this is left out: it takes half a microsecond (a fence over
           // the cluster), 5 % of a product of one round of tiles.
@@ -1223,20 +1216,29 @@ fp4_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
           if (!there) continue;
           if (near) {
 #pragma unroll
-            for (int i = 0; i < 32; i += 4) {
-              const float4 w = *reinterpret_cast<const float4 *>(rows + s0 + h * 32 + i);
-              float *p = &v[h][i];
-              p[0] = p[0] * w.x * rx;
-              p[1] = p[1] * w.y * rx;
-              p[2] = p[2] * w.z * rx;
-              p[3] = p[3] * w.w * rx;
+            for (int i = 0; i < 16; i += 4) {
+              const float4 w = *reinterpret_cast<const float4 *>(rows + s0 + h * 32 + i), q = *reinterpret_cast<const float4 *>(rows + s0 + h * 32 + 16 + i);
+              a[i] = a[i] * w.x * rx;
+              a[i + 1] = a[i + 1] * w.y * rx;
+              a[i + 2] = a[i + 2] * w.z * rx;
+              a[i + 3] = a[i + 3] * w.w * rx;
+              c[i] = c[i] * q.x * rx;
+              c[i + 1] = c[i + 1] * q.y * rx;
+              c[i + 2] = c[i + 2] * q.z * rx;
+              c[i + 3] = c[i + 3] * q.w * rx;
             }
           } else {
 #pragma unroll
-            for (int i = 0; i < 32; ++i) v[h][i] = scaled_far(v[h][i], rows[s0 + h * 32 + i], rx);
+            for (int i = 0; i < 16; ++i) {
+              a[i] = scaled_far(a[i], rows[s0 + h * 32 + i], rx);
+              c[i] = scaled_far(c[i], rows[s0 + h * 32 + 16 + i], rx);
+            }
           }
 #pragma unroll
-          for (int i = 0; i < 32 / PIECE; ++i) put_piece(box, lane, h * (32 / PIECE) + i, &v[h][i * PIECE], TO());
+          for (int i = 0; i < 16 / PIECE; ++i) {
+            put_piece(box, lane, h * (32 / PIECE) + i, a + i * PIECE, TO());
+            put_piece(box, lane, h * (32 / PIECE) + 16 / PIECE + i, c + i * PIECE, TO());
+          }
         }
         if (!there) continue;
         // what hangs over the last column the lanes store, as they do all of a result whose rows do not start on 16 bytes: TMA would round its end
