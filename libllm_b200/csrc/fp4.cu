@@ -1187,9 +1187,8 @@ fp4_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
         constexpr int HALVES = S::BOX / 32, PIECE = 16 / (int)sizeof(TO);                 // 32 features at a time
         const bool last = b == S::BOXES - 1;
         const unsigned box = box0 + turn * S::OUT_BYTES;
-        if (S::BUFFERS == 2) turn ^= 1;
         if (there) {
-          if (lane == 0) {                     // the box's last store has read it
+          if (lane == 0) {                     // the buffer's last store has read it: with two, the newest store reads the other one
             if (S::BUFFERS == 2) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
             else asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
           }
@@ -1251,6 +1250,9 @@ fp4_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
                          ::"l"(&map_out), "r"(f0 + s0), "r"(tok0), "r"(box) : "memory");
             asm volatile("cp.async.bulk.commit_group;" ::: "memory");
           }
+          // Only a store that TMA reads takes its buffer away.  A box that is not there, or that the lanes store, commits no group: with a turn for
+          // each of them the wait above would let the store out of this very buffer stay open.
+          if (S::BUFFERS == 2) turn ^= 1;
         } else {
           __syncwarp();
           const TO *from_box = reinterpret_cast<const TO *>(out_raw + (box - smem_u32(out_raw)));

@@ -383,3 +383,42 @@ def test_offsets_beyond_32_bits():
         out = room[at:].as_strided((300, 300), (step - 4, 1)) if at else room.as_strided((300, 300), (step, 1))
         o.fp4_gemm(q, qw, out=out)
         assert torch.equal(out, want) and int((room != 0).sum()) == int((want != 0).sum())
+
+
+# ---------------------------------------------------------------- several tiles to a CTA
+def whole(rows, K, format, seed, scale=None):
+    """Bfloat16 rows that four bits hold as they are, made on the device: whole numbers up to 6 x 2^2 times the row's power of two (2^scale, or one of eight).
+    The sum over K of the products of two such rows is a whole number below (6 x 4)^2 K times the two powers: exact in 32 bits for K below 29,000, in any
+    order."""
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    b = P.BLOCK[format]
+    n = -(-K // b)
+    kinds = torch.tensor([0., 1, 2, 3, 4, 6, -1, -2, -3, -4, -6], device=DEV, dtype=torch.bfloat16)
+    code = kinds[torch.randint(0, 11, (rows, n, b), generator=g, device=DEV, dtype=torch.int32)]
+    code[:, :, 0] = 6                                        # the block's scale is then the power of two beside it
+    code *= torch.exp2(torch.randint(0, 3, (rows, n, 1), generator=g, device=DEV).float()).bfloat16()
+    e = torch.randint(-4, 4, (rows, 1, 1), generator=g, device=DEV).float() if scale is None else torch.full((rows, 1, 1), float(scale), device=DEV)
+    return (code * torch.exp2(e).bfloat16()).reshape(rows, -1)[:, :K].contiguous()
+
+
+def same_product(M, N, K, format, dtype, seed, x_scale=None, w_scale=None, times=1):
+    """Every element equals the 64-bit product's, narrowed to the result's type."""
+    o = ops()
+    x, w = whole(M, K, format, seed, x_scale), whole(N, K, format, seed + 1, w_scale)
+    qx, qw = o.fp4_quantize(x, format), o.fp4_quantize(w, format)
+    want = (x.double() @ w.double().T).to(dtype)
+    for _ in range(times):
+        out = torch.full((M, N), 7.0, dtype=dtype, device=DEV)
+        o.fp4_gemm(qx, qw, out=out)
+        o.check_tc_status()
+        wrong = out != want
+        assert not wrong.any(), f"{int(wrong.sum())} of {M * N} elements differ, the first at {wrong.nonzero()[0].tolist()}"
+
+
+@pytest.mark.parametrize("M,N,K", [(1030, 16384, 256), (2100, 4099, 256), (600, 16384, 700), (20000, 256, 256), (19200, 1030, 100), (2049, 6000, 2304),
+                                   (600, 128256, 256)])
+@pytest.mark.parametrize("format", FORMATS)
+def test_prompts_into_32_bits_with_several_tiles_to_two_sms(format, M, N, K):
+    """Boxes on their way out lie in two buffers that the next tile writes again: last token tiles that leave warps without tokens, features of which a
+    warp's last box is not there (N % 96 in 64 .. 95) or hangs over."""
+    same_product(M, N, K, format, torch.float32, M + N + K, times=3)
