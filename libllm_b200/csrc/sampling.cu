@@ -132,15 +132,16 @@ __device__ __forceinline__ void draw_from_sorted(const unsigned long long *cand,
     }
     const float r = u * sum;
     float acc = 0.f;
-    int pick = (int)(0xffffffffu - (unsigned)(cand[count - 1] & 0xffffffffull));
-    for (int i = 0; i < count; ++i) {
+    int i = 0;
+    for (; i < count; ++i) {
       acc += probs[i];
-      if (r < acc) {
-        pick = (int)(0xffffffffu - (unsigned)(cand[i] & 0xffffffffull));
-        break;
-      }
+      if (r < acc) break;
     }
-    *out = pick;
+    // u may be 1 in 32 bits: then the last candidate that has a probability at all (minus infinity has none), not one behind it
+    if (i == count)
+      for (--i; i > 0 && probs[i] == 0.f; --i) {
+      }
+    *out = (int)(0xffffffffu - (unsigned)(cand[i] & 0xffffffffull));
   }
 }
 
@@ -278,10 +279,13 @@ sample_kernel(const float *logits, long long stride, int V, float temperature, i
     const float r = u * Z;
     if (tid == 0) result = 0;
     __syncthreads();
-    // The owner of r is the last thread whose running sum before its chunk is <= r
-    // (thread 0 always qualifies); taking the maximum keeps the choice unique even where
-    // rounding makes two neighbouring prefixes equal or out of order by one ulp.
-    if (before <= r && c1 > c0) atomicMax(&result, tid);
+    // The owner of r is the last thread whose running sum before its chunk is <= r, of those whose tokens have
+    // a probability at all (the first of them has 0 before it); taking the maximum keeps the choice unique even where
+    // rounding makes two neighbouring prefixes equal or out of order by one ulp.  The owner's own sum may end
+    // below r, as the next prefix was added up in another order: then its last token that has a probability.
+    // (One of minus infinity, which a mask forbids, has none: of a row of 128,256, half of them masked, one draw in
+    // 27,000 was of a masked token when the last token was taken whatever it had.)
+    if (before <= r && part > 0.f) atomicMax(&result, tid);
     __syncthreads();
     const int owner = result;
     __syncthreads();
@@ -289,8 +293,10 @@ sample_kernel(const float *logits, long long stride, int V, float temperature, i
       float acc = before;
       int pick = c1 - 1;
       for (int i = c0; i < c1; ++i) {
-        acc += expf((row[i] - mx) * inv_t);
-        if (r < acc) { pick = i; break; }
+        const float w = expf((row[i] - mx) * inv_t);
+        acc += w;
+        if (w > 0.f) pick = i;
+        if (r < acc) break;
       }
       out[blockIdx.x] = pick;
     }
