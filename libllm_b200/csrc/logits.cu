@@ -38,17 +38,17 @@ struct Adjust {
   long long ld_allowed;
 };
 
-// A row's penalties.  A division by `rep` is a product with 1 / rep (two roundings of 2^-24 for one: with the division 64 rows of 128,256 took 17.4 us
-// for 16.3, in registers and instructions), in two steps so that 1 / rep is an ordinary number whatever `rep` is.
+// A row's penalties.  A division by `rep` is a product with 1 / rep in 64 bits, narrowed once: two roundings of 2^-53, where the quotient of two numbers of 24 bits lies
+// 2^-49 of itself or more from every border between two others, so that what comes out is the nearest number of 32 bits as the division's would be.
+// (With a product in 32 bits up to a sixth of the quotients were the next number to it, 64 rows of 128,256 took 14.9 us for 15.2; with the division itself, its
+// registers and instructions, 16.6.)
 struct Penalty {
-  float rep, inv, step, pres, freq;
-  __device__ __forceinline__ Penalty(float r, float p, float f) : rep(r), pres(p), freq(f) {
-    step = r < 7.9e-31f ? 1.8446744e19f : r > 1.2e30f ? 5.4210109e-20f : 1.f;        // 2^64, 2^-64 beyond 2^-100 and 2^100
-    inv = 1.f / (r * step);
-  }
+  double inv;
+  float rep, pres, freq;
+  __device__ __forceinline__ Penalty(float r, float p, float f) : inv(1.0 / (double)r), rep(r), pres(p), freq(f) {}
 };
 __device__ __forceinline__ float adjusted(float x, unsigned c, const Penalty &p) {
-  const float said = x > 0.f ? x * p.inv * p.step : x * p.rep;
+  const float said = x > 0.f ? (float)((double)x * p.inv) : x * p.rep;
   const unsigned n = c & ~SEEN;
   x = c ? said : x;
   return n ? x - (p.freq * (float)n + p.pres) : x;

@@ -219,3 +219,23 @@ def test_offsets_beyond_32_bits():
     b.copy_(bias)
     a.copy_(allowed)
     assert torch.equal(o.adjust_logits(logits, bias=b, history=history, lengths=lengths, repetition=1.5, frequency=0.25, allowed=a), want)
+
+
+@pytest.mark.parametrize("repetition", [1.1, 1.2, 1.3, 1.7, 3.0, 0.7, 1.0 + 2.0 ** -23, 1.0 - 2.0 ** -24, 2.0 ** -120 * 1.1, 2.0 ** -99 * 1.3, 2.0 ** 101 * 1.9, 3e38])
+@pytest.mark.parametrize("B,V", [(3, 4000), (40, 2053), (2, 8192)])
+def test_a_division_by_the_repetition_is_rounded_once(repetition, B, V):
+    """A token that occurs and was not drawn has its logit divided or multiplied and nothing else: the nearest number of 32 bits, which is what 64 bits
+    narrow to (their quotient's own rounding, 2^-53, moves none of these across a border: a quotient of two numbers of 24 bits is no border and lies 2^-49 of itself from
+    one at least).  Asked of quotients and products within the ordinary numbers, of logits whose remainders are within them too."""
+    g = torch.Generator().manual_seed(V + 10 * B)
+    exponent = round(math.log2(repetition) / 2)                  # logit and quotient equally far from 1
+    logits = torch.randn(B, V, generator=g) * torch.exp2(torch.randint(-20, 20, (B, V), generator=g).float()) * 2.0 ** exponent
+    history = (~torch.arange(V).int()).expand(B, V).contiguous()
+    got = ops().adjust_logits(logits.to(DEV), history=history.to(DEV), lengths=torch.full((B,), V, dtype=torch.int32, device=DEV),
+                              repetition=torch.full((B,), repetition, device=DEV)).cpu()
+    by = torch.tensor(repetition).double()
+    want = torch.where(logits > 0, logits.double() / by, logits.double() * by).float()
+    asked = (want.abs() >= 2.0 ** -126) & want.isfinite() & (logits.abs() >= 2.0 ** -100)
+    assert asked.float().mean() > 0.3
+    wrong = asked & (got != want)
+    assert not wrong.any(), f"{int(wrong.sum())} of {int(asked.sum())} are not the nearest"
