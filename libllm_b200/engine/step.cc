@@ -40,8 +40,9 @@ bool Engine::GraphKey::operator<(const GraphKey &o) const {
 class Engine::Descriptor {
  public:
   // RowSlot, RowLen, DrawnPos (engines that track histories): a wanted row's slot, the tokens its sequence holds up to it, and where in the sequence a
-  // token drawn from it will stand (-1: it is not the last of the tokens that the step was given).
-  enum Field { Tokens, TokSeq, TokPos, SeqStart, SeqPast, SeqSlot, Want, Uniforms, Fed, RowSlot, RowLen, DrawnPos, Tables };
+  // token drawn from it will stand (-1: it is not the last of the tokens that the step was given).  Repetition, Presence, Frequency (the same engines): the
+  // row's penalties, here and not in a captured step's launches so that other numbers take no other graph.
+  enum Field { Tokens, TokSeq, TokPos, SeqStart, SeqPast, SeqSlot, Want, Uniforms, Fed, RowSlot, RowLen, DrawnPos, Repetition, Presence, Frequency, Tables };
 
   Descriptor() { LLM_CUDA(cudaEventCreateWithFlags(&copied_, cudaEventDisableTiming)); }
   ~Descriptor() { cudaEventDestroy(copied_); }
@@ -53,7 +54,7 @@ class Engine::Descriptor {
     n_want = W;
     this->widths = widths;
     const int H = history ? W : 0;
-    sizes_ = {T, T, T, B + 1, B, B, W, std::max(B, W), T, H, H, H};
+    sizes_ = {T, T, T, B + 1, B, B, W, std::max(B, W), T, H, H, H, H, H, H};
     for (int w : widths) sizes_.push_back(B * w);
     offsets_.assign(1, 0);
     for (int s : sizes_) offsets_.push_back(offsets_.back() + (size_t)((s + 3) / 4 * 4));
@@ -248,7 +249,7 @@ void Engine::validate_adjustments(const std::vector<StepItem> &items, const Samp
 
 // ---------------------------------------------------------------- descriptor
 void Engine::fill(Descriptor &d, const std::vector<Piece> &pieces, const std::vector<StepItem> &items,
-                  const std::vector<int> &want_rows, const float *uniforms, int n_uniforms) {
+                  const std::vector<int> &want_rows, const SamplingParams *sampling, const float *uniforms, int n_uniforms) {
   int *tokens = d.host(Descriptor::Tokens), *tok_seq = d.host(Descriptor::TokSeq), *tok_pos = d.host(Descriptor::TokPos);
   int *seq_start = d.host(Descriptor::SeqStart), *seq_past = d.host(Descriptor::SeqPast), *seq_slot = d.host(Descriptor::SeqSlot);
   int *fed = d.host(Descriptor::Fed);
@@ -292,6 +293,11 @@ void Engine::fill(Descriptor &d, const std::vector<Piece> &pieces, const std::ve
       if (drawn_pos[r] < 0) continue;
       if (drawn_by[(size_t)b] >= 0) drawn_pos[drawn_by[(size_t)b]] = -1;       // the same place asked for twice: the last draw stands
       drawn_by[(size_t)b] = (int)r;
+    }
+    if (sampling && sampling->penalizes()) {
+      std::fill_n((float *)d.host(Descriptor::Repetition), want_rows.size(), sampling->repetition_penalty);
+      std::fill_n((float *)d.host(Descriptor::Presence), want_rows.size(), sampling->presence_penalty);
+      std::fill_n((float *)d.host(Descriptor::Frequency), want_rows.size(), sampling->frequency_penalty);
     }
   }
   if (uniforms) memcpy(d.host(Descriptor::Uniforms), uniforms, sizeof(float) * (size_t)n_uniforms);
@@ -375,10 +381,10 @@ void Engine::sample(const Act &logits, const SamplingParams &s, Descriptor &d, c
       c.places = history_places_;
       c.slots = d.dev(Descriptor::RowSlot);
       c.lengths = d.dev(Descriptor::RowLen);
+      c.repetition = (const float *)d.dev(Descriptor::Repetition);
+      c.presence = (const float *)d.dev(Descriptor::Presence);
+      c.frequency = (const float *)d.dev(Descriptor::Frequency);
     }
-    c.repetition_all = s.repetition_penalty;
-    c.presence_all = s.presence_penalty;
-    c.frequency_all = s.frequency_penalty;
     c.bias = s.logit_bias.empty() ? nullptr : bias_.as<float>();
     c.allowed = allowed_dev;
     c.ld_allowed = (logits.cols + 31) / 32;
@@ -495,7 +501,7 @@ StepResult Engine::run_eager(const std::vector<StepItem> &items, const SamplingP
     Descriptor &d = *eager_desc_[eager_turn_];
     eager_turn_ = (eager_turn_ + 1) % eager_desc_.size();
     d.shape(T, (int)pieces.size(), (int)want_rows.size(), std::vector<int>(cache_->groups().size(), width), opt_.track_history);
-    fill(d, pieces, items, want_rows, uni.data(), (int)uni.size());
+    fill(d, pieces, items, want_rows, sampling, uni.data(), (int)uni.size());
     d.upload(stream_);
     last_h2d_ = (long long)(d.words() * sizeof(int));
     last_d2h_ = 0;
@@ -604,7 +610,7 @@ StepResult Engine::run_decode_graph(const std::vector<StepItem> &items, const Sa
       ++k;
     }
   g.desc.wait_host_free();
-  fill(g.desc, pieces, items, all_rows, uni.data(), B);
+  fill(g.desc, pieces, items, all_rows, sampling, uni.data(), B);
   if (allowed) {
     // a sequence that wants nothing gets no words of its own: what is drawn for it is not handed out
     const size_t n = (size_t)((vocab() + 31) / 32);

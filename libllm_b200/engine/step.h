@@ -49,10 +49,9 @@ struct SamplingParams {
     if (temperature != o.temperature) return temperature < o.temperature;
     if (top_k != o.top_k) return top_k < o.top_k;
     if (top_p != o.top_p) return top_p < o.top_p;
-    if (repetition_penalty != o.repetition_penalty) return repetition_penalty < o.repetition_penalty;
-    if (presence_penalty != o.presence_penalty) return presence_penalty < o.presence_penalty;
-    if (frequency_penalty != o.frequency_penalty) return frequency_penalty < o.frequency_penalty;
-    return logit_bias.empty() && !o.logit_bias.empty();      // the numbers themselves lie in device memory, not in a graph
+    // whether there are penalties and biases; the numbers themselves lie in device memory, not in a graph
+    if (penalizes() != o.penalizes()) return o.penalizes();
+    return logit_bias.empty() && !o.logit_bias.empty();
   }
 };
 
@@ -163,7 +162,7 @@ class Engine {
   void validate(const std::vector<StepItem> &items) const;
   void validate_adjustments(const std::vector<StepItem> &items, const SamplingParams &s) const;
   void fill(Descriptor &d, const std::vector<Piece> &pieces, const std::vector<StepItem> &items, const std::vector<int> &want_rows,
-            const float *uniforms, int n_uniforms);
+            const SamplingParams *sampling, const float *uniforms, int n_uniforms);
   void place_history(Descriptor &d);
   void bring_bias(const SamplingParams &s);
   StepContext context(Descriptor &d, const std::vector<Piece> &pieces, int n_want, bool decode_only, int max_kv_len, Arena *arena,

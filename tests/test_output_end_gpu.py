@@ -339,3 +339,18 @@ def test_the_command_line_takes_penalties_and_an_output_matrix_in_four_bits():
     assert by_command("--head", "nvfp4", "--repetition-penalty", "1.5", "--presence-penalty", "0.5", "--frequency-penalty", "0.25") == want[1]
     bad = subprocess.run([os.path.join(root, "bin", "llm"), "generate", "-m", folder, "--prompt-ids", "1,2", "--head", "fp4"], capture_output=True, text=True, timeout=600)
     assert bad.returncode != 0 and "fp4" in bad.stderr
+
+
+def test_other_penalties_take_no_other_graphs():
+    """Every step may bring penalties of its own: a captured step reads them from its descriptor."""
+    e = engine(track_history=True, max_slots=4)
+    seqs = [Sequence(e.open_sequence()) for _ in range(2)]
+    drawn = run(e, seqs, [tokens_for("C", 12, 21), tokens_for("C", 5, 22)], greedy(repetition_penalty=1.3))
+    before = e.info()["graphs_captured"]
+    for i in range(10):
+        s = greedy(repetition_penalty=1.0 + 0.05 * (i + 1), presence_penalty=0.01 * i, frequency_penalty=0.02 * (10 - i))
+        drawn = run(e, seqs, [[t] for t in drawn], s)
+    assert e.info()["graphs_captured"] - before == 2, "two graphs of the shape take turns, whatever the penalties"
+    for s in (greedy(), greedy(presence_penalty=0.7), greedy(), greedy(repetition_penalty=0.8)):
+        drawn = run(e, seqs, [[t] for t in drawn], s)
+    assert e.info()["graphs_captured"] - before == 4, "two more of steps without penalties"
