@@ -16,7 +16,8 @@ so an edited source is rebuilt and a stale library is never loaded; ``kernels.ma
 same folder tells the host library (and the ``llm`` program, which has no Python around it) where
 each family lies.  While a compiler runs, a line is printed to standard error now and then.
 
-There is no fallback: if a compiler is missing or a build fails, ``ExtensionError`` is raised.
+There is no fallback: if a compiler is missing or a build fails, ``ExtensionError`` is raised.  (Without the torch binding alone its
+calls reach the same kernels through ctypes.)
 
     python -m libllm_b200.csrc.build [family ...]      build kernel families (all by default), the
                                                        host library and the llm program

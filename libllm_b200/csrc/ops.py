@@ -6,6 +6,7 @@ from __future__ import annotations
 
 import ctypes
 import struct
+import sys
 from ctypes import c_char_p, c_float, c_int, c_longlong, c_void_p
 from typing import Optional
 
@@ -90,14 +91,29 @@ def _call_packed(family: str, name: str, args: bytes) -> None:
 
 
 _quick = {}
+_binding = []
+
+
+def _no_quick_call(*args):
+    return None
 
 
 def _quick_call(family: str, name: str, t: torch.Tensor):
     """A function of the torch binding (csrc/torch_calls.cpp), tied to its kernel's library, for calls whose first tensor is ``t``.  It answers
-    None to a call that is not plainly right: the checks here then say what is wrong with it."""
+    None to a call that is not plainly right: the checks here then say what is wrong with it.  Where there is no binding to be had (it takes g++ and
+    torch's headers, which the kernels do not) every call goes through the checks here, to the same kernel, which costs some us of the host."""
     if not t.is_cuda:
-        return lambda *args: None
-    binding = build.load_binding()
+        return _no_quick_call
+    if not _binding:
+        try:
+            _binding.append(build.load_binding())
+        except (ExtensionError, OSError) as e:
+            print(f"[libllm_b200] calls go without the torch binding, some us longer each: {e}", file=sys.stderr, flush=True)
+            _binding.append(None)
+    binding = _binding[0]
+    if binding is None:
+        _quick[name] = _no_quick_call
+        return _no_quick_call
     binding.bind("llm_" + name, ctypes.cast(_fn(family, "llm_" + name, [c_char_p])[0], c_void_p).value)
     f = _quick[name] = getattr(binding, name)
     return f

@@ -123,3 +123,24 @@ def test_matrices_whose_memory_is_not_theirs(kw):
     for call in calls:
         with pytest.raises(InvalidArgError):
             call(changed(**kw))
+
+
+@pytest.mark.parametrize("error", [ExtensionError("no C++ compiler found"), PermissionError("the folder cannot be written")])
+def test_without_the_torch_binding_calls_go_the_longer_way(error, monkeypatch, capsys):
+    """Told once, tried once, and answered with None, upon which every operator goes through its own checks to the kernel."""
+    class OnGpu:
+        is_cuda = True
+
+    tried = []
+
+    def fails():
+        tried.append(1)
+        raise error
+
+    monkeypatch.setattr(ops, "_quick", {})
+    monkeypatch.setattr(ops, "_binding", [], raising=False)
+    monkeypatch.setattr(ops.build, "load_binding", fails)
+    for family, name in (("fp4", "fp4_quantize"), ("fp4", "fp4_gemm"), ("logits", "adjust_logits"), ("fp4", "fp4_quantize")):
+        assert ops._quick_call(family, name, OnGpu())(1, 2, 3) is None
+        assert ops._quick[name](4) is None
+    assert len(tried) == 1 and capsys.readouterr().err.count(str(error)) == 1

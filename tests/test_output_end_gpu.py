@@ -354,3 +354,29 @@ def test_other_penalties_take_no_other_graphs():
     for s in (greedy(), greedy(presence_penalty=0.7), greedy(), greedy(repetition_penalty=0.8)):
         drawn = run(e, seqs, [[t] for t in drawn], s)
     assert e.info()["graphs_captured"] - before == 4, "two more of steps without penalties"
+
+
+def test_operators_without_the_torch_binding(monkeypatch):
+    """The same results by way of ctypes where the binding cannot be had."""
+    from libllm_b200.csrc import ops
+    from libllm_b200.errors import ExtensionError
+
+    def fails():
+        raise ExtensionError("no C++ compiler found")
+
+    g = torch.Generator().manual_seed(30)
+    x, w = (torch.randn(n, 300, generator=g).to(torch.bfloat16).cuda() for n in (5, 70))
+    logits, history = torch.randn(3, 500, generator=g).cuda(), torch.randint(0, 500, (3, 40), generator=g).int().cuda()
+    lengths = torch.tensor([40, 0, 17], dtype=torch.int32).cuda()
+
+    def all_of_them():
+        qx, qw = ops.fp4_quantize(x), ops.fp4_quantize(w)
+        return [qx.codes, qx.row_scale, ops.fp4_dequantize(qw), ops.fp4_gemm(qx, qw), ops.fp4_gemm(qx, qw, out_dtype=torch.bfloat16),
+                ops.adjust_logits(logits, history=history, lengths=lengths, repetition=1.5, presence=0.25)]
+
+    want = all_of_them()
+    monkeypatch.setattr(ops, "_quick", {})
+    monkeypatch.setattr(ops, "_binding", [], raising=False)
+    monkeypatch.setattr(ops.build, "load_binding", fails)
+    assert all(torch.equal(a, b) for a, b in zip(want, all_of_them()))
+    assert ops._binding == [None]
