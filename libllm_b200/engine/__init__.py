@@ -49,7 +49,11 @@ class SamplingParams:
             bias = ()
         elif hasattr(bias, "items"):
             bias = bias.items()
-        object.__setattr__(self, "logit_bias", tuple((int(t), float(v)) for t, v in bias))
+        pairs = tuple((t, int(t), float(v)) for t, v in bias)
+        for t, n, _ in pairs:
+            if not isinstance(t, str) and n != t:
+                raise InvalidArgError(f"logit_bias: {t} is no token id")
+        object.__setattr__(self, "logit_bias", tuple((n, v) for _, n, v in pairs))
 
     def validate(self) -> None:
         _lib.check(_lib.lib().llm_validate_sampling(float(self.temperature), int(self.top_k), float(self.top_p)))

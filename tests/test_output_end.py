@@ -144,3 +144,14 @@ def test_without_the_torch_binding_calls_go_the_longer_way(error, monkeypatch, c
         assert ops._quick_call(family, name, OnGpu())(1, 2, 3) is None
         assert ops._quick[name](4) is None
     assert len(tried) == 1 and capsys.readouterr().err.count(str(error)) == 1
+
+
+def test_token_ids_of_a_bias():
+    import numpy as np
+    from libllm_b200.engine import SamplingParams
+    for bias in ({1: 2}, {"1": 2}, {1.0: 2}, {np.int64(1): 2}, [(1, 2)], ((np.float32(1), 2.0),)):
+        assert SamplingParams(logit_bias=bias).logit_bias == ((1, 2.0),)
+    assert SamplingParams(logit_bias=None).logit_bias == () == SamplingParams(logit_bias={}).logit_bias
+    for bias in ({1.7: 2.0}, [(np.float32(0.5), 1.0)], {-0.5: 1.0}):
+        with pytest.raises(InvalidArgError):
+            SamplingParams(logit_bias=bias)
