@@ -422,3 +422,69 @@ def test_prompts_into_32_bits_with_several_tiles_to_two_sms(format, M, N, K):
     """Boxes on their way out lie in two buffers that the next tile writes again: last token tiles that leave warps without tokens, features of which a
     warp's last box is not there (N % 96 in 64 .. 95) or hangs over."""
     same_product(M, N, K, format, torch.float32, M + N + K, times=3)
+
+
+@pytest.mark.parametrize("M,N,K", [(1030, 16384, 256), (1030, 16384, 1280), (2100, 4099, 256), (2100, 4099, 1280), (2049, 6000, 2304), (300, 40000, 700),
+                                   (20000, 256, 500), (2048, 16384, 2048)])
+@pytest.mark.parametrize("format", FORMATS)
+def test_prompts_with_several_tiles_to_two_sms(format, M, N, K):
+    """Both accumulators, the ring and the places of scales used again from tile to tile: one, two, three, five, eight and nine stages to a tile."""
+    same_product(M, N, K, format, torch.bfloat16, M + N + K)
+    same_product(M, N, K, format, torch.float32, M + N + K + 7)
+
+
+@pytest.mark.parametrize("M,N,K", [(1, 40000, 256), (8, 40000, 2048), (16, 50257, 1111), (17, 40000, 1280), (33, 44444, 700), (64, 40000, 2304),
+                                   (100, 40000, 256), (128, 60000, 1500)])
+@pytest.mark.parametrize("format", FORMATS)
+def test_few_tokens_with_several_tiles_to_an_sm(format, M, N, K):
+    same_product(M, N, K, format, torch.float32, M + N + K)
+    same_product(M, N, K, format, torch.bfloat16, M + N + K + 7)
+
+
+@pytest.mark.parametrize("format", FORMATS)
+def test_an_output_matrix(format):
+    same_product(8, 128256, 2048, format, torch.float32, 1)
+
+
+@pytest.mark.parametrize("M,N,K", [(5, 2048, 4096), (1, 4000, 1800), (16, 1999, 2100), (20, 1000, 8192), (32, 9000, 2048), (1, 512, 16384), (30, 130, 8000),
+                                   (33, 1000, 8192), (100, 600, 9001), (128, 2048, 16384), (64, 1, 7937)])
+@pytest.mark.parametrize("format", FORMATS)
+def test_products_in_parts_of_k(format, M, N, K):
+    """Two, four and eight parts of K, whose sums the CTAs of a cluster hand one another."""
+    same_product(M, N, K, format, torch.float32, M + N + K)
+    same_product(M, N, K, format, torch.bfloat16, M + N + K + 7)
+
+
+@pytest.mark.parametrize("M,N,K", [(5, 2048, 4096), (20, 500, 8192), (100, 600, 9001), (8, 40000, 256), (1030, 16384, 256), (1500, 2000, 700), (20000, 256, 256)])
+@pytest.mark.parametrize("up,down", [(110, -110), (-110, 110), (50, 50), (-55, -55), (-70, -30), (100, -30), (-118, 0), (0, 105)])
+def test_row_scales_at_the_ends_of_the_range(M, N, K, up, down):
+    """In parts of K and in tiles of two SMs, in some rows beside ordinary ones: sums are whole numbers below 2^24 and the powers of two leave them exact, from
+    2^-118 on, to where both are infinite."""
+    o = ops()
+    x, w = whole(M, K, "nvfp4", 1, 0), whole(N, K, "nvfp4", 2, 0)
+    ux, uw = torch.zeros(M, device=DEV), torch.zeros(N, device=DEV)
+    ux[M // 3:], uw[::2] = up, down
+    x, w = x * torch.exp2(ux)[:, None].bfloat16(), w * torch.exp2(uw)[:, None].bfloat16()
+    assert x.isfinite().all() and w.isfinite().all()
+    want = (x.double() @ w.double().T).float()
+    got = o.fp4_gemm(o.fp4_quantize(x), o.fp4_quantize(w))
+    o.check_tc_status()
+    assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("rows,cols", [(50000, 2048), (3000, 1200), (40000, 250), (40000, 500), (50001, 2047), (1200, 16000), (700, 40000)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("format", FORMATS)
+def test_many_rows_into_four_bits_and_back(format, dtype, rows, cols):
+    """Rows that four bits hold as they are come back as they were; and rows that they do not, sampled, are the nearest."""
+    o = ops()
+    x = whole(rows, cols, format, rows + cols).to(dtype)
+    q = o.fp4_quantize(x, format)
+    assert torch.equal(o.fp4_dequantize(q), x.float()) and torch.equal(o.fp4_dequantize(q, torch.bfloat16), x.bfloat16())
+    g = torch.Generator(device=DEV).manual_seed(rows)
+    x = (torch.randn(rows, cols, generator=g, device=DEV) * torch.exp2(torch.randint(-9, 9, (rows, 1), generator=g, device=DEV).float())).to(dtype)
+    q = o.fp4_quantize(x, format)
+    at = torch.randint(0, rows, (20,), generator=torch.Generator().manual_seed(cols)).to(DEV)
+    at[0], at[1] = 0, rows - 1
+    same_values(x[at].cpu(), format, o.fp4_dequantize(q)[at])
+    same_values(x[at].cpu(), format, o.fp4_dequantize(q, torch.bfloat16)[at])
