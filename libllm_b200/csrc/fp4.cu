@@ -597,8 +597,12 @@ __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
-// A sum times its two rows' scales.  Between 2^-63 and 2^63 (`near_one`) either order is safe: sums lie between 2^-20 and 2^40.  Beyond, scales at
-// opposite ends of the range meet first (their product is in range where one step would leave it), scales at the same end one after the other.
+// A sum times its two rows' scales, which are powers of two (mxfp4: 1, so that the order does not matter; what its blocks' scales make of a sum has to lie within 32
+// bits by itself).  nvfp4: codes are multiples of 1/2, block scales of 2^-9, so sums are multiples of 2^-20; a value is 6 x 352 at most, a sum below 2^23 K,
+// 2^51 for the longest K.  Between 2^-63 and 2^64 (`near_one`) either order is safe: sum and first scale meet between 2^-83 and 2^115, without rounding, and the second
+// scale rounds once, if the result leaves the ordinary numbers.  Beyond, scales at opposite ends of the range meet first (their product is in range where
+// one step would leave it).  Scales whose product is out of range go one after the other: both above 1 (rows of 2^117 at most), where a first step that overflows
+// would not have come back, or both below, where a first step that rounds is off by half of 2^-149 and the second makes that less.
 __device__ __forceinline__ bool near_one(float scale) {
   const unsigned e = __float_as_uint(scale) >> 23;       // a NaN or a sign is not near
   return e >= 64 && e <= 190;
@@ -876,6 +880,8 @@ int get_code_map(const void *codes, long long rows, long long K, int box_rows, C
 // enough; beyond, four parts or eight of 32 stages or more.  In 1 / 2 / 4 / 8 parts, us: 2,048 features, K = 2,048, 1 token 5.1 / 4.2 / 3.6 / 3.6, 64 tokens
 // 5.5 / 7.3 / 5.7 / 5.7; K = 1,024, 8 tokens 3.5 / 4.0; K = 8,192, 8 tokens 11.5 / 8.5 / 6.2 / 8.7, 64 tokens 11.9 / 10.9 / 8.0 / 12.3, 128 tokens 13.1 / 14.2 /
 // 10.7 / 17.1; 512 features, K = 16,384, 1 token 19.5 / 12.1 / 8.0 / 5.9; 8,192 features, K = 8,192, 8 tokens 11.9 / 10.4, 64 tokens 12.7 / 13.1.
+// Other parts round their sums elsewhere: of matrices of up to 74 tiles (9,472 features) and K beyond 1,792 a token's result may differ in its last bits between calls of 32
+// and 33 tokens, or of 128 and 129.  Elsewhere it has no part in what other tokens the call holds.
 int k_parts(int M, int N, int K) {
   const long long tiles = (N + FP_ROWS - 1) / FP_ROWS, stages = k_stages(K);
   int parts = 1;

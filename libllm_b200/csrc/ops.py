@@ -653,7 +653,8 @@ def fp4_dequantize(q: Fp4Matrix, dtype: torch.dtype = torch.float32, out: Option
 
 def fp4_gemm(x: Fp4Matrix, w: Fp4Matrix, out: Optional[torch.Tensor] = None, out_dtype: torch.dtype = torch.float32) -> torch.Tensor:
     """out[M, N] = x[M, K] @ w[N, K]^T of two matrices in the same format, on tcgen05 with block scales, 32-bit sums, for any sizes; the
-    result float32 or bfloat16.  A wait inside the kernel that runs out of time is told by ``check_tc_status``."""
+    result float32 or bfloat16.  A wait inside the kernel that runs out of time is told by ``check_tc_status``.  How sums are cut along K goes by the
+    sizes: with K > 1,792 and N <= 9,472 a token's last bits may differ between calls of up to 32, up to 128 and more tokens."""
     if x.format != w.format or x.cols != w.cols:
         raise InvalidArgError(f"fp4_gemm: {x.format} [{x.rows}, {x.cols}] and {w.format} [{w.rows}, {w.cols}] do not meet")
     M, N = x.rows, w.rows

@@ -457,17 +457,18 @@ def test_products_in_parts_of_k(format, M, N, K):
 
 @pytest.mark.parametrize("M,N,K", [(5, 2048, 4096), (20, 500, 8192), (100, 600, 9001), (8, 40000, 256), (1030, 16384, 256), (1500, 2000, 700), (20000, 256, 256)])
 @pytest.mark.parametrize("up,down", [(110, -110), (-110, 110), (50, 50), (-55, -55), (-70, -30), (100, -30), (-118, 0), (0, 105)])
-def test_row_scales_at_the_ends_of_the_range(M, N, K, up, down):
+@pytest.mark.parametrize("format", FORMATS)
+def test_row_scales_at_the_ends_of_the_range(format, M, N, K, up, down):
     """In parts of K and in tiles of two SMs, in some rows beside ordinary ones: sums are whole numbers below 2^24 and the powers of two leave them exact, from
     2^-118 on, to where both are infinite."""
     o = ops()
-    x, w = whole(M, K, "nvfp4", 1, 0), whole(N, K, "nvfp4", 2, 0)
+    x, w = whole(M, K, format, 1, 0), whole(N, K, format, 2, 0)
     ux, uw = torch.zeros(M, device=DEV), torch.zeros(N, device=DEV)
     ux[M // 3:], uw[::2] = up, down
     x, w = x * torch.exp2(ux)[:, None].bfloat16(), w * torch.exp2(uw)[:, None].bfloat16()
     assert x.isfinite().all() and w.isfinite().all()
     want = (x.double() @ w.double().T).float()
-    got = o.fp4_gemm(o.fp4_quantize(x), o.fp4_quantize(w))
+    got = o.fp4_gemm(o.fp4_quantize(x, format), o.fp4_quantize(w, format))
     o.check_tc_status()
     assert torch.equal(got, want)
 
@@ -488,3 +489,16 @@ def test_many_rows_into_four_bits_and_back(format, dtype, rows, cols):
     at[0], at[1] = 0, rows - 1
     same_values(x[at].cpu(), format, o.fp4_dequantize(q)[at])
     same_values(x[at].cpu(), format, o.fp4_dequantize(q, torch.bfloat16)[at])
+
+
+@pytest.mark.parametrize("format", FORMATS)
+@pytest.mark.parametrize("N,K", [(16384, 700), (9500, 2048), (2000, 1792)])
+def test_a_tokens_result_does_not_hang_on_the_others_in_tiles_of_two_sms_either(format, N, K):
+    """Where K is not cut into parts every kernel adds along K in the same order."""
+    o = ops()
+    x, w = rows_like(1301, K, 1).to(DEV), rows_like(N, K, 2).to(DEV)
+    qw = o.fp4_quantize(w, format)
+    whole_call = o.fp4_gemm(o.fp4_quantize(x, format), qw)
+    for n in (1, 16, 17, 33, 100, 129, 257, 600, 1300):
+        assert torch.equal(o.fp4_gemm(o.fp4_quantize(x[:n], format), qw), whole_call[:n]), n
+    o.check_tc_status()
