@@ -415,10 +415,10 @@ StepResult Engine::step(const std::vector<StepItem> &items, const SamplingParams
   }
   // Pages first: either the whole step fits the cache or nothing changes.
   std::vector<std::pair<int, int>> growth;
-  bool decode_only = true;
+  bool decode_only = true;           // and a row for each sequence at most: a captured step has no more
   for (const auto &it : items) {
     growth.push_back({it.slot, cache_->length(it.slot) + (int)it.tokens.size()});
-    decode_only = decode_only && it.tokens.size() == 1;
+    decode_only = decode_only && it.tokens.size() == 1 && it.want.size() <= 1;
   }
   cache_->reserve(growth);
   StepResult out;

@@ -380,3 +380,33 @@ def test_operators_without_the_torch_binding(monkeypatch):
     monkeypatch.setattr(ops.build, "load_binding", fails)
     assert all(torch.equal(a, b) for a, b in zip(want, all_of_them()))
     assert ops._binding == [None]
+
+
+@pytest.mark.parametrize("graphs", [True, False])
+def test_one_place_wanted_twice_in_a_step_of_single_tokens(graphs):
+    """Two draws from the same logits, each with its own uniform number and mask, and the items behind keep theirs."""
+    from libllm_b200.engine import SamplingParams, StepItem
+    e = engine(use_graphs=graphs, track_history=True)
+    V = e.vocab
+    slots = [e.open_sequence() for _ in range(3)]
+    for q in slots:
+        e.step([StepItem(q, tokens_for("C", 4 + q, 31 + q), [])])
+    items = [StepItem(slots[0], [5], [0, 0]), StepItem(slots[1], [6], [0]), StepItem(slots[2], [7], [0, 0, 0])]
+    masks = np.zeros((6, V), dtype=bool)
+    only = [3, V - 1, 40, 31, 32, 0]
+    masks[np.arange(6), only] = True
+    logits, drawn = e.step(items, greedy(repetition_penalty=1.2), None, True, masks)
+    assert drawn.tolist() == only
+    assert np.array_equal(logits[0], logits[1]) and np.array_equal(logits[3], logits[4]) and np.array_equal(logits[3], logits[5])
+    assert not np.array_equal(logits[1], logits[2]) and not np.array_equal(logits[2], logits[3])
+    # without sampling, and by uniform numbers
+    plain = e.step([StepItem(slots[1], [9], [0, 0]), StepItem(slots[0], [8], [0])])
+    assert np.array_equal(plain[0], plain[1]) and not np.array_equal(plain[1], plain[2])
+    s = SamplingParams(1.0, 0, 1.0)
+    u = [0.1, 0.9, 0.4]
+    logits, drawn = e.step([StepItem(slots[1], [9], [0, 0]), StepItem(slots[0], [8], [0])], s, u)
+    p = np.exp(logits.astype(np.float64) - logits.max(axis=1, keepdims=True))
+    cdf = (p / p.sum(axis=1, keepdims=True)).cumsum(axis=1)
+    for r, t in enumerate(drawn):
+        low, high = (cdf[r, t - 1] if t else 0.0), cdf[r, t]
+        assert low - 1e-5 <= u[r] <= high + 1e-5             # a draw's sums round by (V / 1024 + 50) 2^-24 = 3e-6 at most
