@@ -426,6 +426,9 @@ StepResult Engine::step(const std::vector<StepItem> &items, const SamplingParams
     out = run_decode_graph(items, sampling, uniforms, allowed);
   else
     out = run_eager(items, sampling, uniforms, allowed);
+  // where the next step finds the tokens that it is fed by their rows (a captured step whose items all draw has put them there itself)
+  if (out.tokens && out.tokens != last_tokens_.as<int>())
+    LLM_CUDA(cudaMemcpyAsync(last_tokens_.get(), out.tokens, sizeof(int) * (size_t)std::min(out.n_rows, last_capacity_), cudaMemcpyDeviceToDevice, stream_));
   ++steps_run_;
   return out;
 }
@@ -697,8 +700,6 @@ PendingTokens Engine::step_tokens(const std::vector<StepItem> &items, const Samp
     p.done_ = last_graph_->desc.event();
     return p;
   }
-  if (r.tokens != last_tokens_.as<int>())
-    LLM_CUDA(cudaMemcpyAsync(last_tokens_.get(), r.tokens, sizeof(int) * (size_t)n, cudaMemcpyDeviceToDevice, stream_));
   HostTokens &h = token_ring_[token_turn_];
   token_turn_ = (token_turn_ + 1) % token_ring_.size();
   LLM_CUDA(cudaEventSynchronize(h.done));          // its last reader is long gone; this only orders the reuse

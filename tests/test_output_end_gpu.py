@@ -410,3 +410,33 @@ def test_one_place_wanted_twice_in_a_step_of_single_tokens(graphs):
     for r, t in enumerate(drawn):
         low, high = (cdf[r, t - 1] if t else 0.0), cdf[r, t]
         assert low - 1e-5 <= u[r] <= high + 1e-5             # a draw's sums round by (V / 1024 + 50) 2^-24 = 3e-6 at most
+
+
+@pytest.mark.parametrize("graphs", [True, False])
+def test_a_token_fed_by_its_row_is_the_one_that_the_last_sampled_step_drew(graphs):
+    """Whichever call ran that step, and also where not every item of it drew: the same logits, histories and draws as with the tokens' ids."""
+    from libllm_b200.engine import StepItem
+    s = greedy(repetition_penalty=1.4, presence_penalty=0.3, frequency_penalty=0.1)
+    prompts = [tokens_for("C", n, 50 + n) for n in (9, 4, 6)]
+    got = []
+    for by_row in (False, True):
+        e = engine(use_graphs=graphs, track_history=True)
+        slots = [e.open_sequence() for _ in prompts]
+        out = []
+
+        def step(tokens, want, rows=None):
+            items = [StepItem(q, t if rows is None or rows[i] is None or not by_row else [0], [len(t) - 1] if want[i] else [],
+                              None if rows is None or not by_row else rows[i]) for i, (q, t) in enumerate(zip(slots, tokens))]
+            logits, drawn = e.step(items, s)
+            out.append((logits.copy(), drawn.tolist()))
+            return [int(t) for t in drawn]
+
+        d = step(prompts, [True, True, True])
+        d = step([[t] for t in d], [True, True, True], [0, 1, 2])
+        d2 = step([[t] for t in d], [False, True, True], [0, 1, 2])        # rows 0 and 1 are the second's and the third's now
+        d3 = step([[7], [d2[0]], [d2[1]]], [True, False, True], [None, 0, 1])
+        d4 = step([[d3[0]], [8, 9], [d3[1]]], [True, True, True], [0, None, 1])
+        step([[t] for t in d4], [True, True, True], [0, 1, 2])
+        got.append(out)
+    for (la, da), (lb, db) in zip(*got):
+        assert da == db and np.array_equal(la, lb)
