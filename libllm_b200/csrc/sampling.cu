@@ -225,7 +225,7 @@ sample_kernel(const float *logits, long long stride, int V, float temperature, i
   const float *row = logits + (size_t)blockIdx.x * stride;
   const int tid = threadIdx.x;
   const ArgMax top = block_argmax(row, V, sv, si);
-  if (temperature <= 0.f) {
+  if (temperature <= 0.f || top.v == INFINITY) {         // what is infinite has all the probability there is
     if (tid == 0) out[blockIdx.x] = top.i;
     return;
   }
@@ -506,7 +506,7 @@ sample_cluster_kernel(const float *logits, long long stride, int V, float temper
   ArgMax top{-INFINITY, 0x7fffffff};
   for (unsigned q = 0; q < SC; ++q) top = better(top, ArgMax{*in_block(&xmax, q), *in_block(&xidx, q)});
   if (top.i == 0x7fffffff) top.i = 0;
-  if (temperature <= 0.f) {
+  if (temperature <= 0.f || top.v == INFINITY) {         // as in sample_kernel; every block of the cluster has the same `top`
     if (rank == 0 && tid == 0) out[r] = top.i;
     cluster_sync_all();
     return;

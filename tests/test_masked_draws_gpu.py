@@ -63,3 +63,20 @@ def test_the_end_of_the_range(V, top_k, top_p):
     out = torch.empty(n, dtype=torch.int32, device=DEV)
     drawn = ops().sample(row.to(DEV).expand(n, V).contiguous(), 0.7, top_k, top_p, u.to(DEV), out).cpu().long()
     assert allowed[drawn].all(), f"{int((~allowed[drawn]).sum())} of {n} draws are of masked tokens"
+
+
+@pytest.mark.parametrize("top_k,top_p", [(50, 1.0), (1024, 1.0), (50, 0.8), (1, 1.0), (0, 1.0)])
+@pytest.mark.parametrize("V", [331, 20000])
+def test_a_logit_that_a_penalty_took_beyond_32_bits(V, top_k, top_p):
+    """A repetition far below 1 may make logits infinite: such a token stands above every other, the first of several is drawn."""
+    row, allowed = masked_row(V, "half", 4)
+    at = allowed.nonzero().flatten()
+    row[at[7]] = row[at[20]] = 30.0                         # 30 / 1e-38 is beyond 3.4e38
+    history = (~at[[7, 20]].int())[None].contiguous()
+    logits = ops().adjust_logits(row[None].to(DEV), history=history.to(DEV), lengths=torch.tensor([2], dtype=torch.int32, device=DEV), repetition=1e-38)
+    assert logits[0, at[7]] == math.inf and logits[0, at[20]] == math.inf and int(logits.isinf().sum()) == V - len(at) + 2
+    n = 256
+    u = torch.rand(n, generator=torch.Generator().manual_seed(5)).to(DEV)
+    out = torch.empty(n, dtype=torch.int32, device=DEV)
+    drawn = ops().sample(logits.expand(n, V).contiguous(), 0.9, top_k, top_p, u, out)
+    assert (drawn == int(at[7])).all()
